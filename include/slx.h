@@ -197,6 +197,71 @@ slx_status slx_matmul_q30_noalloc(const int64_t* d_a, int M, int K, int dtype, c
 slx_status slx_attention(slx_ctx* ctx, const int64_t* q, const int64_t* k, const int64_t* v, int seq, int q_embd,
                          int kv_dim, int n_heads, int n_kv_heads, int scale_exp, int mode, int window, int64_t* out);
 
+/* ---- float operators -------------------------------------------------------------------------- */
+/* No counterpart in the reference, whose float source runs these steps as separate loops
+ * (Gguf/TransformerEmbeddingSource.cs:143-211): a block's products with their bias, activation, gate and
+ * residual, and the per-head norms of queries and keys with their rotation, each in one pass over device
+ * buffers. Element types carry GGUF's ids (SLX_DTYPE_Q30: GGUF's I64, Q30 integers). The calls queue on
+ * `stream` (NULL = the context's; (void*)1 names CUDA's legacy default stream) on the context's device,
+ * whichever device is current, and may be captured into CUDA graphs. */
+#define SLX_DTYPE_F32 0
+#define SLX_DTYPE_F16 1
+#define SLX_DTYPE_Q30 27
+#define SLX_DTYPE_BF16 30
+#define SLX_ACT_NONE 0
+#define SLX_ACT_RELU 1
+#define SLX_ACT_SILU 2
+#define SLX_ACT_GELU_TANH 3 /* 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
+#define SLX_ACT_GELU_ERF 4  /* 0.5 v (1 + erf(v / sqrt(2))) */
+
+/* y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]; with gate weights
+ * y = act(x . gate^T + gate_bias) * (x . w^T + bias) + residual (the gated FFN's first half).
+ * slx_linear_prepare lays the weights out once, on the context's stream, and waits: the buffers at d_w,
+ * d_gate, d_bias and d_gate_bias (device memory, complete before the call; the biases f32[N], nullable)
+ * may be freed afterwards. dtype is the type of x,
+ * residual and y: F32 takes weights of any GGUF type slx_dequantize decodes, F16 and BF16 weights of their
+ * own type. d_gate NULL: no gate. Sums and the epilogue are fp32, rounded once to dtype.
+ * An F32 product of more than 8 rows runs on the tensor cores from three bf16 parts of every value: a
+ * finite result is as exact as an fp32 sum, an infinite x or w gives an infinity or a NaN.
+ * slx_linear_device: x [M][K], residual (nullable) and y [M][N] with row strides in elements, at least the
+ * row's width; y may be the residual's buffer (same stride) and must not overlap x otherwise. Any M >= 0.
+ * Results do not change from call to call. A bounded wait that gave up is reported by slx_ctx_status
+ * (SLX_ETIMEOUT). info: dtype, N, K, act, gated, device bytes held. */
+typedef struct slx_linear slx_linear;
+slx_status slx_linear_prepare(slx_ctx* ctx, int dtype, const uint8_t* d_w, int64_t w_bytes, int w_dtype, int N, int K,
+                              const float* d_bias, int act, const uint8_t* d_gate, int64_t gate_bytes,
+                              const float* d_gate_bias, slx_linear** out);
+slx_status slx_linear_free(slx_linear* l);
+slx_status slx_linear_info(slx_linear* l, int64_t* info, int n);
+slx_status slx_linear_device(slx_linear* l, const void* d_x, int64_t ldx, int64_t M, const void* d_residual, int64_t ldr,
+                             void* d_y, int64_t ldy, void* stream);
+
+/* Norms of the queries and keys for each head and the rotary positions, in one pass. For a head row x:
+ * u = x / sqrt(mean(x^2) + eps) * w (u = x without a weight), then (u_p, u_{p+h}) for p < h = rot_dim / 2 is
+ * rotated by the angle pos * base^(-2p / rot_dim); values past rot_dim keep u. With SLX_DTYPE_Q30 the
+ * integers are RmsNormPerHead's (Math/IntegerLayerNorm.cs:71-93) followed by ApplyRoPE's
+ * (Math/IntegerAttention.cs:35-58), bit for bit; the causal model's forward runs the same kernel.
+ * slx_rope_create: the table of cos and sin for positions 0..rows-1 (q30 != 0: IntegerRoPECache's Q30
+ * entries; 0: fp32 entries of angles formed in double), shared by any number of layers.
+ * slx_qk_norm_prepare: one layer's heads and norm weights (d_wq, d_wk [head_dim] in device memory, f32, or
+ * int64 for Q30; NULL: that side is rotated only; complete before the call, copied). rot_dim <= head_dim (Q30: equal, eps 0).
+ * slx_qk_norm_rope_device: q [M][heads * head_dim] to qo, k [M][kv_heads * head_dim] to ko, row strides in
+ * elements, at least the row's width; an output may be its input (same stride) and must not overlap the
+ * inputs otherwise. Row m stands at d_pos[m], or at m % T when d_pos is NULL. A position of -1 leaves the
+ * row's outputs as they were; another one outside the table does too and is reported by slx_ctx_status
+ * (SLX_ERANGE). heads or kv_heads may be 0 (its pointers are not read). A table may be freed before the
+ * layers that use it. */
+typedef struct slx_rope slx_rope;
+typedef struct slx_qk_norm slx_qk_norm;
+slx_status slx_rope_create(slx_ctx* ctx, int rows, int rot_dim, float base, int q30, slx_rope** out);
+slx_status slx_rope_free(slx_rope* r);
+slx_status slx_qk_norm_prepare(slx_rope* r, int dtype, int heads, int kv_heads, int head_dim, const void* d_wq,
+                               const void* d_wk, float eps, slx_qk_norm** out);
+slx_status slx_qk_norm_free(slx_qk_norm* h);
+slx_status slx_qk_norm_rope_device(slx_qk_norm* h, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, int64_t M,
+                                   int64_t T, const int32_t* d_pos, void* d_qo, int64_t ldqo, void* d_ko, int64_t ldko,
+                                   void* stream);
+
 /* ---- lattice k-NN search ------------------------------------------------------------------------ */
 /* The embed+search path: EmbeddingLattice<TPayload>(occupants) + QueryKNearestL2(center, k)
  * (Lattice/EmbeddingLattice.cs:70-77) over vectors quantized by EmbeddingAdapter.Quantize

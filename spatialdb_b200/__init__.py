@@ -9,6 +9,8 @@ Host-side mirror of the reference's model sources over the libslx C ABI (include
   forward_causal, next_token, generate (greedy, full re-forward per token).
 * dequantize / read_tensor_f32  (SparseLattice/Gguf/GgufDequantizer.cs, GgufReader.cs).
 * matmul_q30                (SparseLattice/Math/IntegerMatMul.cs) with GGUF-packed weights.
+* Linear, RopeTable, QkNormRope -- float products with bias, activation, gate and residual, and the
+  per-head norms of queries and keys with their rotation (float or Q30), on device buffers.
 
 Tokenizers stay with the caller (the C# host keeps them); these entry points take token ids.
 All work runs in the CUDA library; nothing here computes on the CPU.
@@ -27,6 +29,9 @@ from ._lib import I32P, I64P, F32P, U8P, U64P, VP
  SLX_ESCRATCH) = range(11)
 OPT_WAIT_LIMIT_CYCLES, OPT_TEST_STALL_MMA = 1, 2
 MODEL_ENCODER, MODEL_CAUSAL, MODEL_GEMMA_ENCODER, MODEL_FLOAT_ENCODER = 0, 1, 2, 3
+DTYPE_F32, DTYPE_F16, DTYPE_Q30, DTYPE_BF16 = 0, 1, 27, 30
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU_TANH, ACT_GELU_ERF = range(5)
+STREAM_LEGACY = 1  # CUDA's legacy default stream, the one torch calls stream 0 (0 here: the context's stream)
 
 
 class SlxError(RuntimeError):
@@ -178,6 +183,113 @@ class PreparedWeight:
     def close(self):
         if getattr(self, "_h", None):
             self.ctx._lib.slx_weight_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Linear:
+    """Float matrix product with its epilogue (slx_linear_prepare): y = act(x . w^T + bias) + residual, or
+    with gate weights act(x . gate^T + gate_bias) * (x . w^T + bias) + residual. `dtype` (DTYPE_F32, DTYPE_F16,
+    DTYPE_BF16) is the type of x, residual and y; the weights at the device pointer `d_w` (N rows of K) have
+    GGUF type `w_dtype`, biases are float32. Everything is copied: the buffers may be freed afterwards."""
+
+    def __init__(self, dtype: int, d_w: int, w_bytes: int, w_dtype: int, N: int, K: int, d_bias: int = 0,
+                 act: int = ACT_NONE, d_gate: int = 0, gate_bytes: int = 0, d_gate_bias: int = 0,
+                 ctx: Context | None = None):
+        self.ctx = ctx or Context.default()
+        h = VP()
+        self.ctx.check(self.ctx._lib.slx_linear_prepare(self.ctx._h, int(dtype), VP(d_w or None), int(w_bytes), int(w_dtype),
+                                                        int(N), int(K), VP(d_bias or None), int(act), VP(d_gate or None),
+                                                        int(gate_bytes), VP(d_gate_bias or None), ctypes.byref(h)))
+        self._h = h
+        self.ctx._adopt(self)
+        info = (ctypes.c_int64 * 6)()
+        self.ctx._lib.slx_linear_info(h, info, 6)
+        self.dtype, self.N, self.K, self.act, self.gated, self.device_bytes = list(info)
+        self._call = self.ctx._lib.slx_linear_device
+
+    def apply_device(self, d_x: int, M: int, d_y: int, ldx: int = 0, ldo: int = 0, d_residual: int = 0, ldr: int = 0,
+                     stream: int = 0):
+        """Queue y[M][N] for x[M][K] on device buffers (raw pointers; row strides in elements, 0: the row's
+        width). y may be the residual's buffer."""
+        st = self._call(self._h, d_x, ldx or self.K, M, d_residual or None, ldr or self.N, d_y, ldo or self.N, stream or None)
+        if st:
+            self.ctx.check(st)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self.ctx._lib.slx_linear_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class RopeTable:
+    """cos and sin of positions 0..rows-1 (slx_rope_create): fp32 entries of angles
+    pos * base^(-2p / rot_dim) formed in double, or with q30 the integer IntegerRoPECache
+    (Math/IntegerAttention.cs:14-32). One table serves any number of layers."""
+
+    def __init__(self, rows: int, rot_dim: int, base: float = 10000.0, q30: bool = False, ctx: Context | None = None):
+        self.ctx = ctx or Context.default()
+        h = VP()
+        self.ctx.check(self.ctx._lib.slx_rope_create(self.ctx._h, int(rows), int(rot_dim), float(base), int(q30),
+                                                     ctypes.byref(h)))
+        self._h = h
+        self.ctx._adopt(self)
+        self.rows, self.rot_dim, self.base, self.q30 = int(rows), int(rot_dim), float(base), bool(q30)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self.ctx._lib.slx_rope_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class QkNormRope:
+    """RmsNorm of every query and key head and the rotary positions in one pass (slx_qk_norm_prepare).
+    `dtype` is the rows' type (DTYPE_Q30: int64 Q30, as the causal model's own forward runs it); d_wq and
+    d_wk are device pointers to [head_dim] weights (float32, or int64 for Q30; 0: that side is rotated
+    only), copied."""
+
+    def __init__(self, table: RopeTable, dtype: int, heads: int, kv_heads: int, head_dim: int, d_wq: int = 0,
+                 d_wk: int = 0, eps: float = 0.0):
+        self.ctx = table.ctx
+        h = VP()
+        self.ctx.check(self.ctx._lib.slx_qk_norm_prepare(table._h, int(dtype), int(heads), int(kv_heads), int(head_dim),
+                                                         VP(d_wq or None), VP(d_wk or None), float(eps), ctypes.byref(h)))
+        self._h = h
+        self.ctx._adopt(self)
+        self.dtype, self.heads, self.kv_heads, self.head_dim = int(dtype), int(heads), int(kv_heads), int(head_dim)
+        self._q, self._k = self.heads * self.head_dim, self.kv_heads * self.head_dim
+        self._call = self.ctx._lib.slx_qk_norm_rope_device
+
+    def apply_device(self, d_q: int, d_k: int, M: int, d_qo: int, d_ko: int, T: int = 0, d_pos: int = 0, ldq: int = 0,
+                     ldk: int = 0, ldqo: int = 0, ldko: int = 0, stream: int = 0):
+        """Queue M rows (raw device pointers; row strides in elements, 0: the row's width): q [M][heads][head_dim]
+        to qo, k [M][kv_heads][head_dim] to ko (an output may be its input). Row m stands at the int32 position
+        d_pos[m] (-1: left alone), or without d_pos at m % T (T 0: one sequence of M rows)."""
+        st = self._call(self._h, d_q or None, ldq or self._q, d_k or None, ldk or self._k, M, T or M, d_pos or None,
+                        d_qo or None, ldqo or self._q, d_ko or None, ldko or self._k, stream or None)
+        if st:
+            self.ctx.check(st)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self.ctx._lib.slx_qk_norm_free(self._h)
             self._h = None
 
     def __del__(self):

@@ -557,6 +557,22 @@ bool encode_rows_u16(void* map128, const void* base, int64_t row_u16, int64_t ro
     return r == CUDA_SUCCESS;
 }
 
+bool encode_rows_planes(void* map128, const void* base, int64_t width, int64_t rows, int64_t ld, int planes, int box_k,
+                        int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn || (box_k != 64 && box_k != 32) || width < 1 || rows < 1 || planes < 1 || box_rows < 1 || box_rows > 256)
+        return false;
+    if (((uintptr_t)base & 15) != 0 || (ld * 2) % 16 != 0) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)rows, (cuuint64_t)planes};
+    cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)(ld * rows * 2)};
+    cuuint32_t box[3] = {(cuuint32_t)box_k, (cuuint32_t)box_rows, (cuuint32_t)planes};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn((CUtensorMap*)map128, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box,
+                    estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_k == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS;
+}
+
 void weight_tz(const WDesc& w, int8_t* tz, cudaStream_t st) {
     k_weight_tz<<<(unsigned)w.N, 256, 0, st>>>(w, tz);
 }

@@ -1,0 +1,330 @@
+// k_qk_rope.cu -- RmsNorm of every query and key head and the rotary positions in one pass.
+//
+// Float: for a head row x of hd values, s = 1 / sqrt(sum x^2 / hd + eps), u_j = x_j s w_j; the pair
+// (u_p, u_{p+h}), p < h, becomes (u_p c - u_{p+h} s', u_p s' + u_{p+h} c) with (c, s') the table's entry of the
+// row's position; values past 2 h keep u. All in fp32 from the loaded values to the one rounding at
+// the store. Q30: RmsNormRow, then ApplyRoPE, on int64 values.
+//
+// Both are bound by memory at many rows (every value is read and written once, the table's row once
+// per token) and by latency at one token. A pair's two values belong to one lane, so the rotation
+// needs no exchange, the reduction is the only traffic between lanes, and in-place calls are safe.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "slx_attr.h"
+#include "slx_device.cuh"
+#include "slx_kernels.h"
+#include "slx_qk_rope.h"
+
+namespace slx {
+namespace {
+
+constexpr int QT = 256;  // threads per block
+
+SLX_DEV float to_f(float v) { return v; }
+SLX_DEV float to_f(__half v) { return __half2float(v); }
+SLX_DEV float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+SLX_DEV T from_f(float v);
+template <>
+SLX_DEV float from_f<float>(float v) { return v; }
+template <>
+SLX_DEV __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+SLX_DEV __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <class T>
+struct Vec16 {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+
+// Row m's position, or -1 when the row is to be left alone (a negative entry, or one outside the
+// table, which raises KERR_RANGE unless it is exactly -1).
+SLX_DEV int position(const QkRope& p, int64_t m) {
+    if (!p.pos) return (int)(m % p.T);
+    const int t = p.pos[m];
+    if (t >= 0 && t < p.table_rows) return t;
+    if (t != -1) atomicOr(p.err, KERR_RANGE);
+    return -1;
+}
+
+// 16-byte chunks. Lane j of a head's group of G lanes owns chunk j and its partner chunk j + h for
+// j < h = half / N, and past those the two unrotated chunks 2h + 2(j - h) and the next one. A group walks
+// `iters` heads of one row, so the row's table entries are read once per group.
+template <class T, int G>
+__global__ void __launch_bounds__(QT) k_qk_vec(QkRope p, int slabs, int iters) {
+    constexpr int N = Vec16<T>::N;
+    const int lane = threadIdx.x & 31, j = lane & (G - 1), grp = lane / G;
+    const unsigned gmask = (G == 32 ? 0xffffffffu : (1u << (G & 31)) - 1u) << (grp * G & 31);
+    const int64_t unit = (int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
+    const int64_t m = unit / slabs;
+    if (m >= p.M) return;
+    const int head0 = (int)(unit % slabs) * iters * (32 / G) + grp;
+    const int nheads = p.q.nh + p.k.nh;
+    const int h = p.half / N, chunks = p.hd / N;
+    const bool pair = j < h;
+    const int ca = pair ? j : 2 * j, cb = pair ? j + h : 2 * j + 1;  // 2h + 2(j - h) = 2j
+    const bool has_a = ca < chunks, has_b = cb < chunks;
+    const int pos = position(p, m);
+    if (pos < 0) return;
+    float cs[N], sn[N];
+    if (pair) {
+        const float4* t = (const float4*)(p.table + (int64_t)pos * p.half + (int64_t)j * N);
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const float4 v = t[e / 2];
+            cs[e] = v.x; sn[e] = v.y; cs[e + 1] = v.z; sn[e + 1] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) { cs[e] = 1.0f; sn[e] = 0.0f; }
+    }
+    const float inv_n = 1.0f / (float)p.hd;
+    for (int i = 0; i < iters; i++) {
+        const int head = head0 + i * (32 / G);
+        const bool live = head < nheads;
+        const bool isq = head < p.q.nh;
+        const QkSide& s = isq ? p.q : p.k;
+        const int hh = isq ? head : head - p.q.nh;
+        const T* x = (const T*)s.in + m * s.ld_in + (int64_t)hh * p.hd;
+        Vec16<T> va, vb;
+        float a[N], b[N];
+        if (live && has_a) *(uint4*)&va = *(const uint4*)(x + (int64_t)ca * N);
+        if (live && has_b) *(uint4*)&vb = *(const uint4*)(x + (int64_t)cb * N);
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            a[e] = live && has_a ? to_f(va.v[e]) : 0.0f;
+            b[e] = live && has_b ? to_f(vb.v[e]) : 0.0f;
+        }
+        const float* w = (const float*)s.w;
+        if (w) {  // the same for every lane of a head's group
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; e++) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(gmask, ss, o);
+            const float r = 1.0f / sqrtf(fmaf(ss, inv_n, p.eps));
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                const float4 wa = has_a ? *(const float4*)(w + ca * N + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 wb = has_b ? *(const float4*)(w + cb * N + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                a[e] *= r * wa.x; a[e + 1] *= r * wa.y; a[e + 2] *= r * wa.z; a[e + 3] *= r * wa.w;
+                b[e] *= r * wb.x; b[e + 1] *= r * wb.y; b[e + 2] *= r * wb.z; b[e + 3] *= r * wb.w;
+            }
+        }
+        if (!live) continue;
+        T* y = (T*)s.out + m * s.ld_out + (int64_t)hh * p.hd;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float ya = pair ? fmaf(a[e], cs[e], -(b[e] * sn[e])) : a[e];
+            const float yb = pair ? fmaf(a[e], sn[e], b[e] * cs[e]) : b[e];
+            va.v[e] = from_f<T>(ya);
+            vb.v[e] = from_f<T>(yb);
+        }
+        if (has_a) *(uint4*)(y + (int64_t)ca * N) = *(const uint4*)&va;
+        if (has_b) *(uint4*)(y + (int64_t)cb * N) = *(const uint4*)&vb;
+    }
+}
+
+// Any even head size, rotation width, stride and alignment: one warp per head row, single values. The
+// row is read a second time (from cache) after its norm is known.
+template <class T>
+__global__ void __launch_bounds__(QT) k_qk_any(QkRope p) {
+    const int lane = threadIdx.x & 31, nheads = p.q.nh + p.k.nh;
+    const int64_t unit = (int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
+    const int64_t m = unit / nheads;
+    if (m >= p.M) return;
+    const int head = (int)(unit % nheads);
+    const int pos = position(p, m);
+    if (pos < 0) return;
+    const bool isq = head < p.q.nh;
+    const QkSide& s = isq ? p.q : p.k;
+    const int hh = isq ? head : head - p.q.nh;
+    const T* x = (const T*)s.in + m * s.ld_in + (int64_t)hh * p.hd;
+    T* y = (T*)s.out + m * s.ld_out + (int64_t)hh * p.hd;
+    const float* w = (const float*)s.w;
+    float r = 1.0f;
+    if (w) {
+        float ss = 0.0f;
+        for (int i = lane; i < p.hd; i += 32) {
+            const float v = to_f(x[i]);
+            ss = fmaf(v, v, ss);
+        }
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        r = 1.0f / sqrtf(fmaf(ss, 1.0f / (float)p.hd, p.eps));
+    }
+    const float2* t = p.table + (int64_t)pos * p.half;
+    for (int i = lane; i < p.half; i += 32) {
+        float a = to_f(x[i]), b = to_f(x[i + p.half]);
+        if (w) {
+            a = a * r * w[i];
+            b = b * r * w[i + p.half];
+        }
+        const float2 c = t[i];
+        y[i] = from_f<T>(fmaf(a, c.x, -(b * c.y)));
+        y[i + p.half] = from_f<T>(fmaf(a, c.y, b * c.x));
+    }
+    for (int i = 2 * p.half + lane; i < p.hd; i += 32) {
+        const float a = to_f(x[i]);
+        y[i] = from_f<T>(w ? a * r * w[i] : a);
+    }
+}
+
+template <class T, int G>
+int launch_vec(const QkRope& p, cudaStream_t st) {
+    const int per = 32 / G, nheads = p.q.nh + p.k.nh;
+    const int steps = (nheads + per - 1) / per;  // group steps that cover a row's heads
+    // As many heads to a group as leave about 48 warps to every SM: at one token each group takes one
+    // head (the least latency), at many rows a row's table entries serve all of its heads.
+    const int64_t warps = (int64_t)device_sm_count() * 48;
+    const int iters = (int)std::max<int64_t>(1, std::min<int64_t>(steps, p.M * steps / warps));
+    const int slabs = (steps + iters - 1) / iters;
+    const int64_t units = p.M * slabs;
+    k_qk_vec<T, G><<<(unsigned)((units + QT / 32 - 1) / (QT / 32)), QT, 0, st>>>(p, slabs, iters);
+    return 1;
+}
+
+template <class T>
+int launch_float(const QkRope& p, cudaStream_t st) {
+    constexpr int N = 16 / (int)sizeof(T);
+    auto aligned = [](const QkSide& s) {
+        return s.nh == 0 || (((uintptr_t)s.in | (uintptr_t)s.out) % 16 == 0 && s.ld_in % N == 0 && s.ld_out % N == 0);
+    };
+    const int h = p.half / N, rest = (p.hd - 2 * p.half) / N, lanes = h + (rest + 1) / 2;
+    if (p.half % N == 0 && p.hd % N == 0 && lanes <= 32 && aligned(p.q) && aligned(p.k)) {
+        if (lanes <= 2) return launch_vec<T, 2>(p, st);
+        if (lanes <= 4) return launch_vec<T, 4>(p, st);
+        if (lanes <= 8) return launch_vec<T, 8>(p, st);
+        if (lanes <= 16) return launch_vec<T, 16>(p, st);
+        return launch_vec<T, 32>(p, st);
+    }
+    const int64_t units = p.M * (p.q.nh + p.k.nh);
+    k_qk_any<T><<<(unsigned)((units + QT / 32 - 1) / (QT / 32)), QT, 0, st>>>(p);
+    return 1;
+}
+
+// ---- Q30 -------------------------------------------------------------------------------------------
+
+// RmsNormRow's root for a head's wrapping sum of squares; skip: the row is left as it is (ms <= 0).
+SLX_DEV int64_t q30_root(u128 ss, int n, bool& skip) {
+    skip = (i128)ss < (i128)n;
+    if (skip) return 1;
+    const int64_t r = isqrt_u128(udiv128_u32(ss, (uint32_t)n, ~0ULL / (uint32_t)n));
+    return r == 0 ? 1 : r;
+}
+
+SLX_DEV void q30_rotate(int64_t a, int64_t b, int64_t c, int64_t s, int64_t& ya, int64_t& yb) {
+    ya = lo64(sar128((i128)((u128)((i128)a * c) - (u128)((i128)b * s)), 30));
+    yb = lo64(sar128((i128)((u128)((i128)a * s) + (u128)((i128)b * c)), 30));
+}
+
+// One warp per head row, lane l owning the pairs l, l + 32, ... (PL of them, held in registers).
+template <int PL>
+__global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
+    const int lane = threadIdx.x & 31, nheads = p.q.nh + p.k.nh;
+    const int64_t unit = (int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
+    const int64_t m = unit / nheads;
+    if (m >= p.M) return;
+    const int head = (int)(unit % nheads);
+    const int pos = position(p, m);
+    if (pos < 0) return;
+    const bool isq = head < p.q.nh;
+    const QkSide& s = isq ? p.q : p.k;
+    const int hh = isq ? head : head - p.q.nh;
+    const int64_t* x = (const int64_t*)s.in + m * s.ld_in + (int64_t)hh * p.hd;
+    int64_t* y = (int64_t*)s.out + m * s.ld_out + (int64_t)hh * p.hd;
+    const int64_t* w = (const int64_t*)s.w;
+    const int64_t *cs = p.cs + (int64_t)pos * p.half, *sn = p.sn + (int64_t)pos * p.half;
+    int64_t a[PL], b[PL];
+#pragma unroll
+    for (int e = 0; e < PL; e++) {
+        const int i = lane + 32 * e;
+        a[e] = i < p.half ? x[i] : 0;
+        b[e] = i < p.half ? x[i + p.half] : 0;
+    }
+    bool skip = true;
+    int64_t root = 1;
+    double rd = 1.0;
+    if (w) {
+        u128 ss = 0;
+#pragma unroll
+        for (int e = 0; e < PL; e++) ss += (u128)((i128)a[e] * a[e]) + (u128)((i128)b[e] * b[e]);
+        root = q30_root(warp_sum_u128(ss), p.hd, skip);
+        rd = 1.0 / (double)root;
+    }
+#pragma unroll
+    for (int e = 0; e < PL; e++) {
+        const int i = lane + 32 * e;
+        if (i >= p.half) continue;
+        int64_t u = a[e], v = b[e];
+        if (!skip) {
+            const int64_t wu = w[i], wv = w[i + p.half];
+            u = muldiv_trunc(u, wu, d_i64(wu), root, rd);
+            v = muldiv_trunc(v, wv, d_i64(wv), root, rd);
+        }
+        q30_rotate(u, v, cs[i], sn[i], y[i], y[i + p.half]);
+    }
+}
+
+// Heads wider than the registers of k_qk_q30 hold: the row is read again after its norm is known.
+__global__ void __launch_bounds__(QT) k_qk_q30_wide(QkRope p) {
+    const int lane = threadIdx.x & 31, nheads = p.q.nh + p.k.nh;
+    const int64_t unit = (int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
+    const int64_t m = unit / nheads;
+    if (m >= p.M) return;
+    const int head = (int)(unit % nheads);
+    const int pos = position(p, m);
+    if (pos < 0) return;
+    const bool isq = head < p.q.nh;
+    const QkSide& s = isq ? p.q : p.k;
+    const int hh = isq ? head : head - p.q.nh;
+    const int64_t* x = (const int64_t*)s.in + m * s.ld_in + (int64_t)hh * p.hd;
+    int64_t* y = (int64_t*)s.out + m * s.ld_out + (int64_t)hh * p.hd;
+    const int64_t* w = (const int64_t*)s.w;
+    bool skip = true;
+    int64_t root = 1;
+    double rd = 1.0;
+    if (w) {
+        u128 ss = 0;
+        for (int i = lane; i < p.hd; i += 32) ss += (u128)((i128)x[i] * x[i]);
+        root = q30_root(warp_sum_u128(ss), p.hd, skip);
+        rd = 1.0 / (double)root;
+    }
+    for (int i = lane; i < p.half; i += 32) {
+        int64_t u = x[i], v = x[i + p.half];
+        if (!skip) {
+            u = muldiv_trunc(u, w[i], d_i64(w[i]), root, rd);
+            v = muldiv_trunc(v, w[i + p.half], d_i64(w[i + p.half]), root, rd);
+        }
+        q30_rotate(u, v, p.cs[(int64_t)pos * p.half + i], p.sn[(int64_t)pos * p.half + i], y[i], y[i + p.half]);
+    }
+}
+}  // namespace
+
+int qk_norm_rope(int dtype, const QkRope& p, cudaStream_t st) {
+    if (p.M <= 0 || p.q.nh + p.k.nh <= 0) return 0;
+    if (dtype == DT_F16) return launch_float<__half>(p, st);
+    if (dtype == DT_BF16) return launch_float<__nv_bfloat16>(p, st);
+    return launch_float<float>(p, st);
+}
+
+int qk_norm_rope_q30(const QkRope& p, cudaStream_t st) {
+    if (p.M <= 0 || p.q.nh + p.k.nh <= 0) return 0;
+    const int64_t units = p.M * (p.q.nh + p.k.nh);
+    const unsigned grid = (unsigned)((units + QT / 32 - 1) / (QT / 32));
+    if (p.half <= 32) k_qk_q30<1><<<grid, QT, 0, st>>>(p);
+    else if (p.half <= 64) k_qk_q30<2><<<grid, QT, 0, st>>>(p);
+    else if (p.half <= 128) k_qk_q30<4><<<grid, QT, 0, st>>>(p);
+    else if (p.half <= 256) k_qk_q30<8><<<grid, QT, 0, st>>>(p);
+    else k_qk_q30_wide<<<grid, QT, 0, st>>>(p);
+    return 1;
+}
+
+}  // namespace slx

@@ -318,3 +318,20 @@ SLX_DEV int64_t warp_max_i64(int64_t v) {
     }
     return v;
 }
+
+// floor(v / n) for v < 2^128 and 1 <= n < 2^32 by long division over 32-bit limbs: each step
+// divides (r << 32 | limb) < n * 2^32 with inv = floor((2^64 - 1) / n), an estimate at most two
+// below the quotient.
+SLX_DEV u128 udiv128_u32(u128 v, uint32_t n, uint64_t inv) {
+    u128 q = 0;
+    uint64_t r = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; i--) {
+        const uint64_t cur = (r << 32) | (uint64_t)(uint32_t)(v >> (32 * i));
+        uint64_t qi = __umul64hi(cur, inv);
+        r = cur - qi * n;
+        while (r >= n) { qi++; r -= n; }
+        q |= (u128)qi << (32 * i);
+    }
+    return q;
+}

@@ -47,6 +47,11 @@ bool encode_planes(void* map128, void* base, int64_t kpad, int64_t rows, int pla
                    int box_k = 128);
 // Encodes a TMA map over `rows` rows of row_u16 16-bit elements (no swizzle), box (box_x, box_rows).
 bool encode_rows_u16(void* map128, const void* base, int64_t row_u16, int64_t rows, int box_x, int box_rows);
+// Encodes a TMA map over `planes` planes of `rows` rows of `width` 16-bit elements, `ld` elements apart (a
+// multiple of 8; a plane is rows * ld elements), box (box_k, box_rows, planes), 128-byte swizzle for box_k
+// 64, 64-byte for 32. Elements past width and rows past `rows` read as zero.
+bool encode_rows_planes(void* map128, const void* base, int64_t width, int64_t rows, int64_t ld, int planes, int box_k,
+                        int box_rows);
 // Per-row common trailing zeros of the Q30 composites -> tz[N].
 void weight_tz(const WDesc& w, int8_t* tz, cudaStream_t st);
 // Digits of the widest composite (after the optional per-row shift tz).

@@ -23,84 +23,21 @@
 
 #include "gguf.hpp"
 #include "slx.h"
+#include "slx_ctx.h"
 #include "slx_kernels.h"
 #include "slx_gemm.h"
 #include "slx_search.h"
 #include "slx_tree.h"
 #include "slx_vocab.h"
 #include "slx_float.h"
+#include "slx_qk_rope.h"
 
 using namespace slx;
 
-// Kernel classes reported by slx_profile_end.
-enum KClass { KC_GEMM, KC_ATTENTION, KC_NORM, KC_ROPE, KC_FFN_GATE, KC_EMBED, KC_POOL, KC_ADD, KC_ARGMAX, KC_GEMV,
-              KC_SPLIT, KC_FALLBACK, KC_SEARCH, KC_VOCAB, KC_COUNT };
 static const char* kKClassName[KC_COUNT] = {"gemm", "attention", "norm", "rope", "ffn_gate", "embed", "pool", "add",
                                             "argmax", "gemv", "split", "fallback", "search", "vocab"};
 
-struct ProfRecord {
-    int cls;
-    int launches;
-    cudaEvent_t a, b;
-    double macs, bytes, tc_macs;
-};
-
-struct slx_ctx {
-    int device = 0;
-    cudaStream_t stream = nullptr;
-    std::string err;
-    int* d_flag = nullptr;
-    int64_t launches = 0;            // kernels queued by the library on this context
-    bool prof = false;
-    std::vector<ProfRecord> records;
-    GemmWorkspace kws;               // scratch of the kernel-level matmul entry points
-    WaitOptions wait;                // bounded-wait settings of the tensor-core GEMMs (slx_ctx_set_option)
-    std::atomic<int> refs{1};        // slx_destroy's reference plus one per live model, weight and lattice
-    std::vector<cudaEvent_t> event_pool;
-    cudaEvent_t event() {
-        if (!event_pool.empty()) { cudaEvent_t e = event_pool.back(); event_pool.pop_back(); return e; }
-        cudaEvent_t e = nullptr;
-        cudaEventCreate(&e);
-        return e;
-    }
-};
-
-// Runs one launcher (which returns how many kernels it queued), counting launches and, when
-// profiling, bracketing it with events on the launch stream.
-template <class F>
-static inline void run_k(slx_ctx* c, int cls, double macs, double bytes, cudaStream_t st, F&& f, double tc_macs = 0) {
-    if (!c->prof) {
-        c->launches += f();
-        return;
-    }
-    ProfRecord r{cls, 0, c->event(), c->event(), macs, bytes, tc_macs};
-    cudaEventRecord(r.a, st);
-    r.launches = f();
-    cudaEventRecord(r.b, st);
-    c->launches += r.launches;
-    c->records.push_back(r);
-}
-
 namespace {
-
-int set_err(slx_ctx* c, int code, const char* fmt, ...) {
-    if (!c) return code;
-    char buf[1024];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    c->err = buf;
-    return code;
-}
-
-#define CK(call)                                                                                 \
-    do {                                                                                         \
-        cudaError_t e_ = (call);                                                                 \
-        if (e_ != cudaSuccess)                                                                   \
-            return set_err(ctx, e_ == cudaErrorMemoryAllocation ? SLX_EOOM : SLX_ECUDA, "%s: %s", \
-                           #call, cudaGetErrorString(e_));                                      \
-    } while (0)
 
 struct DevBuf {
     void* p = nullptr;
@@ -117,9 +54,11 @@ int64_t isqrt64_host(int64_t v) {
     return x;
 }
 
+}  // namespace
+
 // IntegerRoPECache (Math/IntegerAttention.cs:14-32): built on the host in double precision with
 // the C library's pow/cos/sin, truncated to Q30.
-void rope_table(int rows, int hd, float base, std::vector<int64_t>& cs, std::vector<int64_t>& sn) {
+void slx::rope_table(int rows, int hd, float base, std::vector<int64_t>& cs, std::vector<int64_t>& sn) {
     int half = hd / 2;
     cs.assign((size_t)rows * half, 0);
     sn.assign((size_t)rows * half, 0);
@@ -136,8 +75,6 @@ void rope_table(int rows, int hd, float base, std::vector<int64_t>& cs, std::vec
             sn[(size_t)t * half + i] = q30(std::sin(angle));
         }
 }
-
-}  // namespace
 
 struct slx_model {
     slx_ctx* ctx = nullptr;
@@ -812,12 +749,10 @@ int check_flag(slx_ctx* ctx, cudaStream_t st) {
     CK(cudaMemcpyAsync(&flag, ctx->d_flag, sizeof(int), cudaMemcpyDeviceToHost, st));
     CK(cudaMemsetAsync(ctx->d_flag, 0, sizeof(int), st));
     CK(cudaStreamSynchronize(st));
-    if (flag & KERR_RANGE) return set_err(ctx, SLX_ERANGE, "index out of range (token id and UNK row outside the table)");
+    if (flag & KERR_RANGE) return set_err(ctx, SLX_ERANGE, "index out of range (token id and UNK row outside the table, or a position outside the RoPE table)");
     if (flag & KERR_TIMEOUT) return set_err(ctx, SLX_ETIMEOUT, "a tensor-core GEMM gave up on a bounded wait");
     return SLX_OK;
 }
-
-cudaStream_t pick(slx_ctx* ctx, void* s) { return s ? (cudaStream_t)s : ctx->stream; }
 
 int encode_eager(slx_model* m, const int32_t* d_ids, int B, int T, int64_t* d_pooled, cudaStream_t st);
 
@@ -951,6 +886,22 @@ void to_float_l2(const int64_t* v, int d, int sb, float* out) {
 
 }  // namespace
 
+// Drops one reference; the last one frees the context. Models, weights and lattices hold one each,
+// so the context (its device, stream and error word) outlives every object created on it, whatever
+// order the host frees them in (a garbage-collected host may finalize the context first).
+void slx::ctx_release(slx_ctx* ctx) {
+    if (ctx->refs.fetch_sub(1) != 1) return;
+    cudaSetDevice(ctx->device);
+    if (ctx->stream) cudaStreamSynchronize(ctx->stream);
+    cudaFree(ctx->d_flag);
+    for (auto& r : ctx->records) { cudaEventDestroy(r.a); cudaEventDestroy(r.b); }
+    for (cudaEvent_t e : ctx->event_pool) cudaEventDestroy(e);
+    gemm_workspace_free(ctx->kws);
+    if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
+    if (ctx->stream) cudaStreamDestroy(ctx->stream);
+    delete ctx;
+}
+
 // ==============================================================================================
 // extern "C" ABI
 // ==============================================================================================
@@ -971,21 +922,6 @@ slx_status slx_init(int device, slx_ctx** out) {
     c->kws.wait = &c->wait;
     *out = c.release();
     return SLX_OK;
-}
-
-// Drops one reference; the last one frees the context. Models, weights and lattices hold one each,
-// so the context (its device, stream and error word) outlives every object created on it, whatever
-// order the host frees them in (a garbage-collected host may finalize the context first).
-static void ctx_release(slx_ctx* ctx) {
-    if (ctx->refs.fetch_sub(1) != 1) return;
-    cudaSetDevice(ctx->device);
-    if (ctx->stream) cudaStreamSynchronize(ctx->stream);
-    cudaFree(ctx->d_flag);
-    for (auto& r : ctx->records) { cudaEventDestroy(r.a); cudaEventDestroy(r.b); }
-    for (cudaEvent_t e : ctx->event_pool) cudaEventDestroy(e);
-    gemm_workspace_free(ctx->kws);
-    if (ctx->stream) cudaStreamDestroy(ctx->stream);
-    delete ctx;
 }
 
 slx_status slx_destroy(slx_ctx* ctx) {
