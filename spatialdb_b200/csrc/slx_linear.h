@@ -34,7 +34,7 @@ struct Plan {
     int nkb() const { return (K + bk() - 1) / bk(); }
     int64_t block_bytes() const { return (int64_t)planes() * TR * bk() * 2; }
     int tiles_n() const { return (N + TR - 1) / TR; }
-    int64_t tile_bytes() const { return (int64_t)tiles_n() * nkb() * block_bytes(); }
+    int64_t tile_bytes() const { return (int64_t)(tiles_n() + 1) / 2 * 2 * nkb() * block_bytes(); }  // a pair of tiles at a time
     int64_t k4() const { return (K + 3) / 4 * 4; }
 };
 

@@ -145,10 +145,11 @@ def test_activations(ctx, dtype, act, M):
 
 
 @pytest.mark.parametrize("dtype,M,K,N", [("bf16", 2500, 512, 2304), ("f16", 1111, 768, 3000), ("f32", 1500, 512, 1500),
-                                         ("bf16", 512, 2048, 6000)])
+                                         ("bf16", 512, 2048, 6000), ("f32", 2000, 300, 1500), ("f16", 5001, 100, 1111),
+                                         ("bf16", 300, 64, 10001), ("f32", 4099, 33, 1027)])
 def test_persistent_tiles(ctx, dtype, M, K, N):
-    """More tiles than SMs: every CTA walks several, the accumulators in turn."""
-    Case(ctx, dtype, M, K, N, act="silu", bias=True, residual=True).check()
+    """More tiles than SMs: every CTA, or pair of CTAs, walks several, the accumulators in turn."""
+    Case(ctx, dtype, M, K, N, act="silu", bias=True, residual=True, pad=8).check()
     Case(ctx, dtype, M, K, N, act="silu", gated=True).check()
 
 
