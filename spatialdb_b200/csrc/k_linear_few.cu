@@ -71,8 +71,9 @@ __device__ __forceinline__ uint4 load_x8(const FewParams& p, int m, int k) {
 template <class T>
 __device__ __forceinline__ void finish(const FewParams& p, int m, int n, float acc, float gacc, bool gated) {
     float v = acc + (p.bias ? p.bias[n] : 0.0f);
-    if (gated) v *= activate(gacc + (p.gbias ? p.gbias[n] : 0.0f), p.act);
-    else v = activate(v, p.act);
+    float a[1] = {gated ? gacc + (p.gbias ? p.gbias[n] : 0.0f) : v};
+    activate_all<T>(a, p.act);
+    v = gated ? v * a[0] : a[0];
     if (p.r) v += to_f(((const T*)p.r)[(int64_t)m * p.ldr + n]);
     ((T*)p.y)[(int64_t)m * p.ldo + n] = from_f<T>(v);
 }

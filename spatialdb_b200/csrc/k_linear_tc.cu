@@ -4,9 +4,9 @@
 // A tile is 128 weight rows a CTA (one TMEM lane each) x NT activation rows (the MMA's N). Weights are
 // laid out once in the swizzled blocks that the MMA reads, so a K block of a tile is one contiguous
 // copy; activations come through a TMA tensor map on the caller's rows (a packed copy when their base
-// or stride is not a multiple of 16 bytes). Warp 0 loads, warp 1 issues the MMAs, eight warps run the
+// or stride is not a multiple of 16 bytes). Warp 0 loads, warp 1 issues the MMAs, 16 warps run the
 // epilogue: 16 columns at a time go from TMEM through shared memory, so that bias, activation, gate,
-// residual and the one rounding run on eight consecutive outputs of a row with 16-byte accesses.
+// residual and the one rounding run on runs of a row's outputs with vector accesses.
 //
 // f32 (PLANES = 3): each value is the exact sum of three bf16 parts (8 significant bits each, by
 // truncation), x = x1 + x2 + x3. x1 w1 goes to one accumulator, the corrections x1 w2 + x2 w1 + x2 w2 +
@@ -14,19 +14,24 @@
 // truncates when it adds to an accumulator, which biases long sums, so every 256 values of K both
 // accumulators are added to fp32 registers (rounded to nearest) and started anew.
 //
-// Three forms, by the number of tiles:
-//   SPLIT   fewer tiles than SMs: a cluster of up to 8 CTAs shares a tile, each with a range of the K
-//           blocks. CTA c of S adds columns c NT / S... of all partial sums, in rank order, over
-//           distributed shared memory, and finishes them. One launch, no workspace, the same result every time.
-//   SINGLE  persistent, one CTA per SM, the epilogue of a tile under the MMAs of the next (two accumulators).
-//   PAIR    persistent, two CTAs (cta_group::2) on 256 weight rows: each loads its own 128 weight rows and
-//           half of the activation rows, which halves the activation bytes per MMA.
+// Two forms, the cheaper by an estimate of its cycles (choose):
+//   ONE   one tile at a time. A cluster of S = 1, 2, 4 or 8 CTAs shares the tile, each with a range of the K
+//         blocks, so that few tiles still occupy the SMs. CTA c of S finishes columns c NT / S...: the others
+//         store their partial sums of them into its shared memory, and it adds them in rank order. One
+//         launch, no workspace, the same result every time. The epilogue's warps have nothing to do before the
+//         sums are there: f32 rows, and 16-bit rows TMA cannot address, are loaded, split and swizzled by
+//         them (MANUAL), without a pass of its own.
+//   PAIR  persistent, two CTAs (cta_group::2) on 256 weight rows: each loads its own 128 weight rows and half
+//         of the activation rows, which halves the activation bytes per MMA; the epilogue of a tile runs
+//         under the MMAs of the next (two accumulators).
 // Every mbarrier wait is bounded.
 #include <cuda.h>
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "slx_attr.h"
 #include "slx_device.cuh"
@@ -41,13 +46,13 @@ namespace {
 
 using namespace tc;
 
-enum Mode { SINGLE = 0, SPLIT = 1, PAIR = 2 };
+enum Mode { ONE = 0, PAIR = 1 };
 
-constexpr int EPI = 8;                      // epilogue warps: two per TMEM lane quarter
+constexpr int EPI = 16;                     // epilogue warps: four groups of one warp per TMEM lane quarter
+constexpr int GROUPS = EPI / 4;
 constexpr int LT = 32 * (2 + EPI);          // threads
 constexpr int SMEM_MAX = 227 * 1024;
 constexpr int CHUNK = 8;                    // f32: K blocks (of 32) between promotions to registers
-constexpr int SLAB = 16;                    // columns the epilogue moves through shared memory at a time
 constexpr int GROUP_M = 8;                  // activation tiles walked together (their rows stay in L2)
 
 struct TcParams {
@@ -56,8 +61,10 @@ struct TcParams {
     const void* r;
     void* y;
     int64_t ldr, ldo;
-    int M, N, nkb, act, f16, vec;
-    int tiles_n, tiles_m, tiles, split;
+    const void* x;   // MANUAL: the caller's rows
+    int64_t ldx;
+    int M, N, K, nkb, act, f16, vec;
+    int tiles_n, tiles_m, tiles, log2_split;
     int* err;
     long long wait_limit;
     int stall_mma;
@@ -72,12 +79,15 @@ struct Shape {
     static constexpr int STAGE = S * WB + PLANES * XR * ROWB;
     static constexpr int ACC = S * (PLANES == 3 ? 2 : 1);      // accumulators of NT columns
     static constexpr int COLS = 2 * ACC * NT;                  // two buffers
-    static constexpr int OUT = 2 * S * SLAB * TR * 4;          // epilogue staging, both groups of four warps
+    static constexpr int HC = NT / GROUPS;                     // columns of an epilogue group
+    static constexpr int SLAB = HC < 16 || PLANES == 3 || GATED ? 8 : 16;  // columns it moves through shared memory at a time
+    // the epilogue's shared memory: the groups' staging, or in ONE the partial sums this CTA finishes
+    static constexpr int OUT = MODE == ONE ? S * NT * TR * 4 : GROUPS * S * SLAB * TR * 4;
     static constexpr int FIT = (SMEM_MAX - 1024 - 512 - OUT) / STAGE;
     static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+    static constexpr int GROUPS_X = XR * (ROWB / 16) / 32;     // MANUAL: groups of 32 chunks of eight values a block
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + OUT + 1024 + 512;
     static_assert(COLS <= 512 && STAGES >= 2, "tile does not fit");
-    static_assert((size_t)S * NT * TR * 4 <= (size_t)STAGES * STAGE || MODE != SPLIT, "split partials reuse the stages");
 };
 
 template <int CG>
@@ -132,21 +142,20 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// All 32 lanes of every warp of the cluster arrive, and wait before they arrive again.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
     return a;
 }
-__device__ __forceinline__ float4 peer_ld4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
+__device__ __forceinline__ void peer_st(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ void peer_arrive(uint32_t addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
@@ -157,76 +166,98 @@ __device__ __forceinline__ uint32_t idesc_f16(int m, int n, int bf16) {
     return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// Eight consecutive outputs n.. of row m from their sums (and gate sums): the epilogue proper.
-template <class T>
-struct Eight {
-    float r[8];  // residual
-    bool vec, any;
+// A thread's share of a tile's outputs: of rows m of y, the values of four weight rows n.. and of four more
+// from n + 64 (a warp's reads of the staged sums then fall on different banks, and its stores are runs of
+// 128 bytes or more). FAST: the tile lies inside y and rows take vectors of four values.
+template <class T, bool GATED>
+struct Columns {
+    float b[8], gb[8];
+    int n;
 
-    __device__ __forceinline__ void load(const TcParams& p, int64_t m, int n) {
-        any = m < p.M && n < p.N;
-        vec = any && p.vec && n + 8 <= p.N;
+    __device__ __forceinline__ void begin(const TcParams& p, int first) {
+        n = first;
+        fill(b, p.bias, p.N);
+        if (GATED) fill(gb, p.gbias, p.N);
+    }
+    __device__ __forceinline__ int at(int j) const { return n + (j & 3) + (j >> 2) * 64; }
+    __device__ __forceinline__ void fill(float (&v)[8], const float* from, int N) const {
 #pragma unroll
-        for (int j = 0; j < 8; j++) r[j] = 0.0f;
-        if (!p.r || !any) return;
-        const T* src = (const T*)p.r + m * p.ldr + n;
-        if (vec) {
-            uint4 raw[sizeof(T) / 2];
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = ((const uint4*)src)[i];
-#pragma unroll
-            for (int j = 0; j < 8; j++) r[j] = to_f(((const T*)raw)[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (n + j < p.N) r[j] = to_f(src[j]);
-        }
+        for (int j = 0; j < 8; j++) v[j] = from && at(j) < N ? from[at(j)] : 0.0f;
     }
 
-    __device__ __forceinline__ void store(const TcParams& p, int64_t m, int n, float (&v)[8], float (&g)[8], bool gated) {
-        if (!any) return;
-        const bool full = n + 8 <= p.N;
-        if (p.bias) add8(v, p.bias, n, p.N, full);
-        if (gated && p.gbias) add8(g, p.gbias, n, p.N, full);
-        float(&a)[8] = gated ? g : v;
-        switch (p.act) {
-            case ACT_RELU: each<ACT_RELU>(a); break;
-            case ACT_SILU: each<ACT_SILU>(a); break;
-            case ACT_GELU_TANH: each<ACT_GELU_TANH>(a); break;
-            case ACT_GELU_ERF: each<ACT_GELU_ERF>(a); break;
-            default: break;
-        }
-        T o[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = from_f<T>((gated ? g[j] * v[j] : v[j]) + r[j]);
-        T* dst = (T*)p.y + m * p.ldo + n;
-        if (vec) {
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; i++) ((uint4*)dst)[i] = ((const uint4*)o)[i];
-        } else {
+    struct Four {
+        T v[4];
+    };
+    struct __align__(16) Residual {
+        Four f[2];
+    };
+    template <bool FAST>
+    __device__ __forceinline__ void load(const TcParams& p, int64_t m, Residual& r) const {
+        if (!p.r) return;
+        const T* src = (const T*)p.r + m * p.ldr;
+        if (FAST) {
+            copy(&r.f[0], src + n);
+            copy(&r.f[1], src + n + 64);
+        } else if (m < p.M) {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (n + j < p.N) dst[j] = o[j];
+                if (at(j) < p.N) r.f[j >> 2].v[j & 3] = src[at(j)];
         }
     }
-
-    static __device__ __forceinline__ void add8(float (&v)[8], const float* b, int n, int N, bool full) {
-        if (full) {  // n is a multiple of 8 and the vector is 16-byte aligned
-            const float4 x = *(const float4*)(b + n), y = *(const float4*)(b + n + 4);
-            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-            v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    // Items' sums (and gate sums) to outputs, R rows of m apart `step`.
+    template <bool FAST, int R>
+    __device__ __forceinline__ void store(const TcParams& p, int64_t m, int step, float (&v)[8 * R], float (&g)[8 * R],
+                                          const Residual (&r)[R]) const {
+#pragma unroll
+        for (int j = 0; j < 8 * R; j++) {
+            v[j] += b[j & 7];
+            if (GATED) g[j] += gb[j & 7];
+        }
+        if (GATED) {
+            activate_all<T>(g, p.act);
+#pragma unroll
+            for (int j = 0; j < 8 * R; j++) v[j] *= g[j];
         } else {
+            activate_all<T>(v, p.act);
+        }
+        if (p.r) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (n + j < N) v[j] += b[n + j];
+            for (int j = 0; j < 8 * R; j++) v[j] += to_f(r[j >> 3].f[(j >> 2) & 1].v[j & 3]);
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int64_t row = m + i * step;
+            T* dst = (T*)p.y + row * p.ldo;
+            Four o[2];
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j >> 2].v[j & 3] = from_f<T>(v[8 * i + j]);
+            if (FAST) {
+                copy(dst + n, &o[0]);
+                copy(dst + n + 64, &o[1]);
+            } else if (row < p.M) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (at(j) < p.N) dst[at(j)] = o[j >> 2].v[j & 3];
+            }
         }
     }
-    template <int ACT>
-    static __device__ __forceinline__ void each(float (&v)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = activate(v[j], ACT);
+    static __device__ __forceinline__ void copy(void* dst, const void* src) {  // four values
+        if (sizeof(T) == 4) *(uint4*)dst = *(const uint4*)src;
+        else *(uint2*)dst = *(const uint2*)src;
     }
 };
+
+// C consecutive accumulator columns of this thread's lane.
+template <int C>
+__device__ __forceinline__ void tmem_cols(uint32_t at, float (&v)[C]) {
+    static_assert(C == 8 || C == 16, "columns");
+    uint32_t a[C];
+    if constexpr (C == 16) tmem_ld16(at, a);
+    else tmem_ld8(at, a);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < C; j++) v[j] = __uint_as_float(a[j]);
+}
 
 // Tile t as (activation tile, weight tile): weight tiles slowest inside groups of GROUP_M activation tiles, so
 // that the CTAs at work share both operands in L2.
@@ -238,7 +269,135 @@ __device__ __forceinline__ void tile_at(const TcParams& p, int tiles_n, int t, i
     tn = i / width;
 }
 
+__device__ __forceinline__ uint16_t bf16_cut(float v) { return (uint16_t)(__float_as_uint(v) >> 16); }
+
+// The three bf16 parts of an fp32 value, each the leading eight significant bits of what is left
+// (truncated, so no part overflows): their sum is the value exactly. A value that is not finite keeps
+// itself in the first part (a NaN stays one) and zeros in the others.
+__device__ __forceinline__ void split3(float v, uint16_t (&o)[3]) {
+    o[0] = bf16_cut(v);
+    o[1] = o[2] = 0;
+    if (!isfinite(v)) {
+        if (isnan(v)) o[0] |= 0x40;
+        return;
+    }
+    const float r1 = v - __uint_as_float((uint32_t)o[0] << 16);
+    o[1] = bf16_cut(r1);
+    o[2] = bf16_cut(r1 - __uint_as_float((uint32_t)o[1] << 16));
+}
+
+// Eight values of a row from column k, zeros past K: as few and wide loads as the address allows.
+__device__ __forceinline__ uint4 row8(const uint16_t* row, int k, int K) {
+    const uint16_t* src = row + k;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (k + 8 <= K) {
+        if (((uintptr_t)src & 15) == 0) return *(const uint4*)src;
+        if (((uintptr_t)src & 3) == 0) {
+            const uint32_t* s4 = (const uint32_t*)src;
+            return make_uint4(s4[0], s4[1], s4[2], s4[3]);
+        }
+    }
+    uint16_t e[8];
+    *(uint4*)e = v;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (k + j < K) e[j] = src[j];
+    return *(const uint4*)e;
+}
+__device__ __forceinline__ void row8(const float* row, int k, int K, float (&f)[8]) {
+    const float* src = row + k;
+    if (k + 8 <= K && ((uintptr_t)src & 15) == 0) {
+        *(float4*)f = *(const float4*)src;
+        *(float4*)(f + 4) = *(const float4*)(src + 4);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = k + j < K ? src[j] : 0.0f;
+    }
+}
+
+// Eight values of one chunk of x, on their way from the caller's rows to a stage.
+template <int PLANES>
+struct Chunk {
+    uint4 v;
+    __device__ __forceinline__ void load(const TcParams& p, int64_t m, int k) {
+        v = m < p.M ? row8((const uint16_t*)p.x + m * p.ldx, k, p.K) : make_uint4(0, 0, 0, 0);
+    }
+    // Chunk c of row r of a stage's activation area: 128-byte rows, chunks XORed with r % 8.
+    __device__ __forceinline__ void store(uint32_t area, int rows, int r, int c) const {
+        const uint32_t at = area + r * 128 + ((c ^ (r & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    }
+};
+template <>
+struct Chunk<3> {
+    float f[8];
+    __device__ __forceinline__ void load(const TcParams& p, int64_t m, int k) {
+        if (m < p.M) {
+            row8((const float*)p.x + m * p.ldx, k, p.K, f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] = 0.0f;
+        }
+    }
+    // The three parts' planes of 64-byte rows, chunks XORed with (r / 2) % 4.
+    __device__ __forceinline__ void store(uint32_t area, int rows, int r, int c) const {
+        uint16_t e[3][8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            uint16_t o[3];
+            split3(f[j], o);
+#pragma unroll
+            for (int q = 0; q < 3; q++) e[q][j] = o[q];
+        }
+#pragma unroll
+        for (int q = 0; q < 3; q++) {
+            const uint32_t at = area + q * rows * 64 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+            const uint4 w = *(const uint4*)e[q];
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+        }
+    }
+};
+
+// MANUAL: the epilogue's warps fill the stages' activation areas. A warp takes every LW-th group of 32
+// chunks (a group lies in one K block), the next group's values in flight while it stores this one's; a
+// stage's full barrier counts its groups. LW is such that a warp has a group in at least every ST-th block:
+// when it waits for block n's stage it then knows block n - 2 ST consumed (it has waited for a later one), so
+// the parity it waits for cannot be an older phase's.
 template <class T, int NT, int PLANES, bool GATED, int MODE>
+__device__ bool load_rows(const TcParams& p, int m0, int kb0, int kb1, int w, int lane, uint32_t sbase, uint32_t full0,
+                          uint32_t empty0, long long limit) {
+    using Sh = Shape<NT, PLANES, GATED, MODE>;
+    constexpr int PER = Sh::ROWB / 16, ST = Sh::STAGES;  // chunks of a row in a block
+    constexpr int LW = Sh::GROUPS_X * ST < EPI ? Sh::GROUPS_X * ST : EPI;
+    static_assert(Sh::GROUPS_X >= EPI || LW % Sh::GROUPS_X == 0, "a warp's groups lie LW / GROUPS_X blocks apart");
+    if (w >= LW) return true;
+    const int groups = (kb1 - kb0) * Sh::GROUPS_X;
+    Chunk<PLANES> buf[2];
+    auto fetch = [&](Chunk<PLANES>& c, int g) {
+        const int i = (g % Sh::GROUPS_X) * 32 + lane;
+        if (g < groups) c.load(p, m0 + i / PER, (kb0 + g / Sh::GROUPS_X) * (Sh::ROWB / 2) + i % PER * 8);
+    };
+    auto put = [&](const Chunk<PLANES>& c, int g) {
+        const int i = (g % Sh::GROUPS_X) * 32 + lane, n = g / Sh::GROUPS_X, s = n % ST;
+        if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((uint32_t)(n / ST) & 1u) ^ 1u, limit))) return false;
+        c.store(sbase + s * Sh::STAGE + Sh::S * Sh::WB, Sh::XR, i / PER, i % PER);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full0 + 8 * s);
+        return true;
+    };
+    fetch(buf[0], w);
+    for (int g = w; g < groups; g += 2 * LW) {
+        fetch(buf[1], g + LW);
+        if (!put(buf[0], g)) return false;
+        if (g + LW >= groups) break;
+        fetch(buf[0], g + 2 * LW);
+        if (!put(buf[1], g + LW)) return false;
+    }
+    return true;
+}
+
+template <class T, int NT, int PLANES, bool GATED, int MODE, bool MANUAL>
 __global__ void __launch_bounds__(LT, 1)
 k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmg,
             const __grid_constant__ TcParams p) {
@@ -261,7 +420,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     if (threadIdx.x == 0) {
         s_fail = 0;
         for (int i = 0; i < ST; i++) {
-            mbar_init(full0 + 8 * i, 1);
+            mbar_init(full0 + 8 * i, MANUAL ? 1 + Sh::GROUPS_X : 1);
             mbar_init(empty0 + 8 * i, 1);
         }
         for (int b = 0; b < 2; b++) {
@@ -283,17 +442,19 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     }
     fence_before();
     __syncthreads();
-    if (MODE == PAIR) cluster_sync();  // both CTAs' barriers exist before either is signalled
+    if (MODE == PAIR) cluster_sync();   // both CTAs' barriers exist before either is signalled
+    if (MODE == ONE) cluster_arrive();  // waited for before the first store to another CTA
+    bool met = false;
     fence_after();
     const uint32_t tmem = *tmem_slot, sbase = smem_u32(smem);
 
     // This CTA's tiles and K blocks.
-    const int rank = MODE == SINGLE ? 0 : (int)cluster_rank();
+    const int rank = (int)cluster_rank(), split = 1 << p.log2_split;
     const int tiles_n = MODE == PAIR ? (p.tiles_n + 1) / 2 : p.tiles_n;
-    const int tile0 = MODE == SPLIT ? (int)blockIdx.x / p.split : (int)blockIdx.x / CG;
-    const int tstep = MODE == SPLIT ? p.tiles : (int)gridDim.x / CG;
-    const int kb0 = MODE == SPLIT ? (int)((int64_t)p.nkb * rank / p.split) : 0;
-    const int kb1 = MODE == SPLIT ? (int)((int64_t)p.nkb * (rank + 1) / p.split) : p.nkb;
+    const int tile0 = MODE == ONE ? (int)blockIdx.x >> p.log2_split : (int)blockIdx.x / CG;
+    const int tstep = MODE == ONE ? p.tiles : (int)gridDim.x / CG;
+    const int kb0 = MODE == ONE ? (int)(((int64_t)p.nkb * rank) >> p.log2_split) : 0;
+    const int kb1 = MODE == ONE ? (int)(((int64_t)p.nkb * (rank + 1)) >> p.log2_split) : p.nkb;
     constexpr int CH = PLANES == 3 ? CHUNK : 1 << 30;
 
     if (warp == 0) {
@@ -321,10 +482,10 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                         if (GATED) pair_load_2d(dst + Sh::WB, &tmg, 0, line, lead);
                         pair_load_3d(dst + S * Sh::WB, &tmx, kb * (ROWB / 2), m0, 0, lead);
                     } else {
-                        mbar_expect_tx(bar, Sh::STAGE);
+                        mbar_expect_tx(bar, MANUAL ? S * Sh::WB : Sh::STAGE);
                         bulk_load(dst, p.w + (blk0 + kb) * Sh::WB, Sh::WB, bar);
                         if (GATED) bulk_load(dst + Sh::WB, p.g + (blk0 + kb) * Sh::WB, Sh::WB, bar);
-                        tma_load_3d(dst + S * Sh::WB, &tmx, kb * (ROWB / 2), m0, 0, bar);
+                        if (!MANUAL) tma_load_3d(dst + S * Sh::WB, &tmx, kb * (ROWB / 2), m0, 0, bar);
                     }
                     if (++s == ST) { s = 0; ph ^= 1u; }
                 }
@@ -393,12 +554,14 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                 }
             }
         }
-    } else {  // epilogue: two groups of four warps, each half of the tile's columns; thread = weight row (TMEM lane)
+    } else {  // epilogue: groups of four warps, each a quarter of the tile's columns; thread = weight row (TMEM lane)
         const int q4 = warp & 3, part = (warp - 2) >> 2, row = 32 * q4 + lane;
-        constexpr int HC = NT / 2;  // columns of a group
+        constexpr int HC = Sh::HC, SLAB = Sh::SLAB;
         const uint32_t tbase = tmem + ((uint32_t)(32 * q4) << 16) + part * HC;
         const uint32_t free0 = MODE == PAIR ? peer_addr(tfree0, 0) : tfree0;
         float* st = out_stage + part * S * SLAB * TR;
+        const int tid = (int)threadIdx.x - 64 - 128 * part, col = tid >> 4;
+        const float* src = st + col * TR + (tid & 15) * 4;
         int use = 0;
         auto release = [&](int buf) {  // this warp has read the buffer
             fence_before();
@@ -413,6 +576,10 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
             tile_at(p, tiles_n, t, tm, tn);
             const int64_t m0 = (int64_t)tm * NT + part * HC;
             const int n0 = (MODE == PAIR ? 2 * tn + rank : tn) * TR;
+            Columns<T, GATED> out;
+            out.begin(p, n0 + (tid & 15) * 4);
+            if (MANUAL && !load_rows<T, NT, PLANES, GATED, MODE>(p, tm * NT, kb0, kb1, warp - 2, lane, sbase, full0, empty0, limit))
+                s_fail = 1;  // the wait below runs out too
             float acc[PLANES == 3 ? S : 1][PLANES == 3 ? HC : 1];  // f32: the promoted sums
             bool ok = true;
             int chunks = 0;
@@ -428,131 +595,136 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
 #pragma unroll
                     for (int v = 0; v < S; v++)
 #pragma unroll
-                        for (int c = 0; c < HC; c += 16) {
-                            uint32_t a[16], k[16];
+                        for (int c = 0; c < HC; c += SLAB) {
+                            float a[SLAB], k[SLAB];
                             const uint32_t at = tbase + (buf * Sh::ACC + 2 * v) * NT + c;
-                            tmem_ld16(at, a);
-                            tmem_ld16(at + NT, k);
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            tmem_cols<SLAB>(at, a);
+                            tmem_cols<SLAB>(at + NT, k);
 #pragma unroll
-                            for (int j = 0; j < 16; j++) {
-                                const float sum = __uint_as_float(a[j]) + __uint_as_float(k[j]);
-                                acc[v][c + j] = chunks ? acc[v][c + j] + sum : sum;
-                            }
+                            for (int j = 0; j < SLAB; j++) acc[v][c + j] = chunks ? acc[v][c + j] + (a[j] + k[j]) : a[j] + k[j];
                         }
                     release(buf);
                 }
             }
-            // A warp that gave up still takes the barriers of its group, so that none waits for it.
             const int buf = (use - 1) & 1;
-            if (MODE == SPLIT) {  // this CTA's partial sums, [v][column][weight row], over the stages (all consumed)
-                float* sums = (float*)smem;
-                if (ok) {
+            if (MODE == ONE) {  // partial sums to the CTAs that finish the columns: [v][column of the part][source][weight row]
+                cluster_wait();  // every CTA of the cluster is running
+                met = true;
+                if (!ok) break;
+                const int sh = __popc(NT - 1) - p.log2_split, cols = 1 << sh;
+                const uint32_t base = smem_u32(out_stage) + (uint32_t)(rank * TR + row) * 4;
 #pragma unroll
-                    for (int v = 0; v < S; v++)
+                for (int v = 0; v < S; v++)
 #pragma unroll
-                        for (int c = 0; c < HC; c += 16) {
-                            float* dst = sums + ((int64_t)v * NT + part * HC + c) * TR + row;
-                            uint32_t a[16];
-                            if (PLANES == 1) {
-                                tmem_ld16(tbase + (buf * Sh::ACC + v) * NT + c, a);
-                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                            }
+                    for (int c = 0; c < HC; c += SLAB) {
+                        float a[SLAB];
+                        if (PLANES == 1) tmem_cols<SLAB>(tbase + (buf * Sh::ACC + v) * NT + c, a);
+                        const int k0 = part * HC + c;
+                        if (tm * NT + k0 >= p.M) break;  // columns past the last row of x
 #pragma unroll
-                            for (int j = 0; j < 16; j++) dst[j * TR] = PLANES == 1 ? __uint_as_float(a[j]) : acc[v][PLANES == 1 ? 0 : c + j];
+                        for (int j = 0; j < SLAB; j++) {
+                            const int k = k0 + j;
+                            const uint32_t at = base + (((v << sh) + (k & (cols - 1))) << p.log2_split) * (TR * 4);
+                            peer_st(peer_addr(at, k >> sh), PLANES == 1 ? a[j] : acc[v][PLANES == 1 ? 0 : c + j]);
                         }
-                }
+                    }
             } else {
-                const int tid = (int)threadIdx.x - 64 - 128 * part;
-                auto slab = [&](int c) {
-                    Eight<T> e[2];
-#pragma unroll
-                    for (int i = 0; i < 2; i++) e[i].load(p, m0 + c + 8 * i + (tid >> 4), n0 + (tid & 15) * 8);
-#pragma unroll
-                    for (int v = 0; v < S; v++) {
-                        uint32_t a[16];
-                        if (PLANES == 1) {
-                            tmem_ld16(tbase + (buf * Sh::ACC + v) * NT + c, a);
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        }
-#pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            st[(v * SLAB + j) * TR + row] = PLANES == 1 ? __uint_as_float(a[j]) : acc[v][PLANES == 1 ? 0 : c + j];
-                    }
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-#pragma unroll 1
-                    for (int i = 0; i < 2; i++) {
-                        const float* src = st + (8 * i + (tid >> 4)) * TR + (tid & 15) * 8;
-                        // the two 16-byte halves in an order that keeps eight lanes on different banks
-                        const int h = (tid >> 2) & 1;
-                        float v[8], g[8];
-                        const float4 a = *(const float4*)(src + 4 * h), b = *(const float4*)(src + 4 * (h ^ 1));
-                        *(float4*)v = h ? b : a;
-                        *(float4*)(v + 4) = h ? a : b;
-                        if (GATED) {
-                            const float4 ga = *(const float4*)(src + SLAB * TR + 4 * h), gb = *(const float4*)(src + SLAB * TR + 4 * (h ^ 1));
-                            *(float4*)g = h ? gb : ga;
-                            *(float4*)(g + 4) = h ? ga : gb;
-                        }
-                        if (i == 0) e[0].store(p, m0 + c + (tid >> 4), n0 + (tid & 15) * 8, v, g, GATED);
-                        else e[1].store(p, m0 + c + 8 + (tid >> 4), n0 + (tid & 15) * 8, v, g, GATED);
-                    }
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                };
-                // whole group or nothing: a warp whose wait ran out takes the others with it
+                // whole group or nothing: a warp whose wait ran out takes the others with it, so that none is
+                // left at a barrier
                 int alive;
                 asm volatile("{\n .reg .pred q, r;\n setp.ne.b32 q, %1, 0;\n bar.red.and.pred r, %2, 128, q;\n selp.b32 %0, 1, 0, r;\n}\n"
                              : "=r"(alive)
                              : "r"((int)ok), "r"(1 + part)
                              : "memory");
                 if (!alive) break;
-                if (PLANES == 1) {
+                auto slab = [&](int c, auto fast) {
+                    constexpr bool FAST = decltype(fast)::value;
+                    constexpr int R = SLAB / 8;
+                    typename Columns<T, GATED>::Residual res[R];
+#pragma unroll
+                    for (int i = 0; i < R; i++) out.template load<FAST>(p, m0 + c + 8 * i + col, res[i]);
+#pragma unroll
+                    for (int v = 0; v < S; v++) {
+                        float a[SLAB];
+                        if (PLANES == 1) tmem_cols<SLAB>(tbase + (buf * Sh::ACC + v) * NT + c, a);
+#pragma unroll
+                        for (int j = 0; j < SLAB; j++)
+                            st[(v * SLAB + j) * TR + row] = PLANES == 1 ? a[j] : acc[v][PLANES == 1 ? 0 : c + j];
+                    }
+                    if (PLANES == 1 && c + SLAB == HC) release(buf);
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
+                    float v[8 * R], g[8 * R];
+#pragma unroll
+                    for (int i = 0; i < 2 * R; i++) {
+                        *(float4*)(v + 4 * i) = *(const float4*)(src + (i >> 1) * 8 * TR + (i & 1) * 64);
+                        if (GATED) *(float4*)(g + 4 * i) = *(const float4*)(src + (SLAB + (i >> 1) * 8) * TR + (i & 1) * 64);
+                    }
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
+                    out.template store<FAST, R>(p, m0 + c + col, 8, v, g, res);
+                };
+                if (p.vec && n0 + TR <= p.N && m0 + HC <= p.M) {
+                    if (PLANES == 1) {
 #pragma unroll 1
-                    for (int c = 0; c < HC; c += SLAB) slab(c);
-                    release(buf);
+                        for (int c = 0; c < HC; c += SLAB) slab(c, std::true_type{});
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < HC; c += SLAB) slab(c, std::true_type{});
+                    }
+                } else if (PLANES == 1) {
+#pragma unroll 1
+                    for (int c = 0; c < HC; c += SLAB) slab(c, std::false_type{});
                 } else {
 #pragma unroll
-                    for (int c = 0; c < HC; c += SLAB) slab(c);
+                    for (int c = 0; c < HC; c += SLAB) slab(c, std::false_type{});
                 }
             }
-            if (!ok) break;
         }
     }
     fence_before();
+    __syncwarp();
+    if (MODE == ONE && !met) cluster_wait();
+    Columns<T, GATED> last;
+    typename Columns<T, GATED>::Residual res[1];
+    const int chunk = (int)threadIdx.x & 15, first = ((int)threadIdx.x - 64) >> 4;
+    int tm = 0, tn = 0;
+    int64_t mr = 0;
+    bool fast = false;
+    if (MODE == ONE && warp >= 2) {  // what the finish needs besides the sums, asked for before they are there
+        tile_at(p, tiles_n, tile0, tm, tn);
+        last.begin(p, tn * TR + chunk * 4);
+        fast = p.vec && (tn + 1) * TR <= p.N;
+        mr = (int64_t)tm * NT + rank * (NT >> p.log2_split);
+        if (fast && mr + first < p.M) last.template load<true>(p, mr + first, res[0]);
+    }
     __syncthreads();
-    if (MODE == SPLIT) {
-        cluster_sync();  // every CTA's partial sums are in its shared memory (or it failed and said so)
-        if (!s_fail && warp >= 2) {
-            const int cols = NT / p.split;
-            int tm, tn;
-            tile_at(p, tiles_n, tile0, tm, tn);
-            for (int i = (int)threadIdx.x - 64; i < cols * (TR / 8); i += EPI * 32) {
-                const int c = rank * cols + (i >> 4), n = tn * TR + (i & 15) * 8;
-                const int64_t m = (int64_t)tm * NT + c;
-                Eight<T> e;
-                e.load(p, m, n);
-                if (!e.any) continue;
-                float v[8], g[8];
+    cluster_sync();  // ONE: all partial sums have arrived; PAIR: no CTA leaves while the other signals it
+    if (MODE == ONE && !s_fail && warp >= 2) {
+        const int cols = NT >> p.log2_split;
+        for (int i = first; i < cols; i += EPI * 2) {
+            const int64_t m = mr + i;
+            if (m >= p.M) break;
+            if (!fast) last.template load<false>(p, m, res[0]);
+            else if (i != first) last.template load<true>(p, m, res[0]);
+            float v[8], g[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = g[j] = 0.0f;
-                const uint32_t at = sbase + (uint32_t)(c * TR + (i & 15) * 8) * 4;
-                for (int q = 0; q < p.split; q++) {
-                    const uint32_t from = peer_addr(at, q);
+            for (int j = 0; j < 8; j++) v[j] = g[j] = 0.0f;
+            const float* src = out_stage + (int64_t)i * split * TR + chunk * 4;
+#pragma unroll 4
+            for (int q = 0; q < split; q++) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const float4 a = peer_ld4(from + 16 * h);
-                        v[4 * h] += a.x; v[4 * h + 1] += a.y; v[4 * h + 2] += a.z; v[4 * h + 3] += a.w;
-                        if (GATED) {
-                            const float4 b = peer_ld4(from + NT * TR * 4 + 16 * h);
-                            g[4 * h] += b.x; g[4 * h + 1] += b.y; g[4 * h + 2] += b.z; g[4 * h + 3] += b.w;
-                        }
+                for (int h = 0; h < 2; h++) {
+                    const float4 a = *(const float4*)(src + q * TR + 64 * h);
+                    v[4 * h] += a.x; v[4 * h + 1] += a.y; v[4 * h + 2] += a.z; v[4 * h + 3] += a.w;
+                    if (GATED) {
+                        const float4 b = *(const float4*)(src + (cols * split + q) * TR + 64 * h);
+                        g[4 * h] += b.x; g[4 * h + 1] += b.y; g[4 * h + 2] += b.z; g[4 * h + 3] += b.w;
                     }
                 }
-                e.store(p, m, n, v, g, GATED);
             }
+            if (fast) last.template store<true, 1>(p, m, 0, v, g, res);
+            else last.template store<false, 1>(p, m, 0, v, g, res);
         }
     }
-    if (MODE != SINGLE) cluster_sync();  // no CTA leaves while another reads its memory or signals its barriers
     if (s_fail && threadIdx.x == 0 && p.err) atomicOr(p.err, KERR_TIMEOUT);
     if (warp == 1) {
         fence_after();
@@ -562,23 +734,6 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
 }
 
 // ---- layouts ----------------------------------------------------------------------------------------
-
-__device__ __forceinline__ uint16_t bf16_cut(float v) { return (uint16_t)(__float_as_uint(v) >> 16); }
-
-// The three bf16 parts of an fp32 value, each the leading eight significant bits of what is left
-// (truncated, so no part overflows): their sum is the value exactly. A value that is not finite keeps
-// itself in the first part (a NaN stays one) and zeros in the others.
-__device__ __forceinline__ void split3(float v, uint16_t (&o)[3]) {
-    o[0] = bf16_cut(v);
-    o[1] = o[2] = 0;
-    if (!isfinite(v)) {
-        if (isnan(v)) o[0] |= 0x40;
-        return;
-    }
-    const float r1 = v - __uint_as_float((uint32_t)o[0] << 16);
-    o[1] = bf16_cut(r1);
-    o[2] = bf16_cut(r1 - __uint_as_float((uint32_t)o[1] << 16));
-}
 
 // One thread per 16-byte chunk of the tiles.
 __global__ void k_tiles16(const uint16_t* __restrict__ w, int N, int K, int nkb, int64_t chunks, uint4* __restrict__ out) {
@@ -627,15 +782,8 @@ __global__ void k_split_x(const float* __restrict__ x, int64_t ldx, int64_t M, i
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t m = i / (kp / 8);
         const int k = (int)(i % (kp / 8)) * 8;
-        const float* src = x + m * ldx + k;
         float f[8];
-        if (k + 8 <= K && ((uintptr_t)src & 15) == 0) {
-            *(float4*)f = *(const float4*)src;
-            *(float4*)(f + 4) = *(const float4*)(src + 4);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) f[j] = k + j < K ? src[j] : 0.0f;
-        }
+        row8(x + m * ldx, k, K, f);
         uint16_t e[3][8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -655,22 +803,12 @@ __global__ void k_pack_x(const uint16_t* __restrict__ x, int64_t ldx, int64_t M,
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t m = i / (kp / 8);
         const int k = (int)(i % (kp / 8)) * 8;
-        uint16_t e[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = k + j < K ? x[m * ldx + k + j] : (uint16_t)0;
-        *(uint4*)(out + m * kp + k) = *(const uint4*)e;
+        *(uint4*)(out + m * kp + k) = row8(x + m * ldx, k, K);
     }
 }
 
-unsigned grid_for(int64_t items) { return (unsigned)std::min<int64_t>((items + 255) / 256, (int64_t)device_sm_count() * 16); }
-
-int kp_of(const Plan& p) { return p.planes() == 3 ? p.nkb() * 32 : (p.K + 7) / 8 * 8; }
-
-bool tma_rows(const Plan& p, const Call& c) {  // the caller's 16-bit rows as they are
-    return p.planes() == 1 && (uintptr_t)c.x % 16 == 0 && c.ldx % 8 == 0;
-}
-
-// Clusters of `size` CTAs that can be resident at once (a GPC with an odd number of SMs leaves one out).
+// Clusters of `size` CTAs of a kernel that can be resident at once (a GPC whose SMs are not a multiple of the
+// size leaves some out). Asked once per kernel and size: the library is built for one GPU.
 int resident_clusters(const void* fn, size_t smem, int size) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(device_sm_count() / size * size));
@@ -683,11 +821,8 @@ int resident_clusters(const void* fn, size_t smem, int size) {
     cfg.attrs = at;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) {
-        cudaGetLastError();
-        return 0;
-    }
-    return n;
+    if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) cudaGetLastError();
+    return std::max(n, 1);
 }
 
 struct Operands {
@@ -696,13 +831,17 @@ struct Operands {
     int width;  // 16-bit values of a row that hold data
 };
 
-template <class T, int NT, int PLANES, bool GATED, int MODE>
-bool launch(const Plan& pl, const Call& c, const Operands& op, int split, cudaStream_t st) {
+template <class T, int NT, int PLANES, bool GATED, int MODE, bool MANUAL>
+bool launch(const Plan& pl, const Call& c, const Operands& op, int log2_split, cudaStream_t st) {
     using Sh = Shape<NT, PLANES, GATED, MODE>;
-    auto* fn = k_linear_tc<T, NT, PLANES, GATED, MODE>;
+    auto* fn = k_linear_tc<T, NT, PLANES, GATED, MODE, MANUAL>;
     if (ensure_smem((const void*)fn, Sh::SMEM) != cudaSuccess) return false;
     CUtensorMap tmx, tmw, tmg;
-    if (!tc::encode_rows_planes(&tmx, op.x, op.width, c.M, op.ldx, PLANES, pl.bk(), Sh::XR)) return false;
+    if (MANUAL) {
+        std::memset(&tmx, 0, sizeof tmx);
+    } else if (!tc::encode_rows_planes(&tmx, op.x, op.width, c.M, op.ldx, PLANES, pl.bk(), Sh::XR)) {
+        return false;
+    }
     if (MODE == PAIR) {  // the weights' blocks as lines of 128 bytes, swizzled already
         const int64_t lines = pl.tile_bytes() / 128;
         if (!tc::encode_rows_u16(&tmw, pl.tiles, 64, lines, 64, Sh::WB / 128)) return false;
@@ -714,34 +853,32 @@ bool launch(const Plan& pl, const Call& c, const Operands& op, int split, cudaSt
     TcParams p;
     p.w = pl.tiles; p.g = pl.gtiles; p.bias = pl.bias; p.gbias = pl.gbias;
     p.r = c.r; p.y = c.y; p.ldr = c.ldr; p.ldo = c.ldo;
-    p.M = (int)c.M; p.N = pl.N; p.nkb = pl.nkb(); p.act = pl.act; p.f16 = pl.dtype == DT_F16;
-    constexpr int PER = 16 / (int)sizeof(T);
-    p.vec = (uintptr_t)c.y % 16 == 0 && c.ldo % PER == 0 && (!c.r || ((uintptr_t)c.r % 16 == 0 && c.ldr % PER == 0));
+    p.x = c.x; p.ldx = c.ldx;
+    p.M = (int)c.M; p.N = pl.N; p.K = pl.K; p.nkb = pl.nkb(); p.act = pl.act; p.f16 = pl.dtype == DT_F16;
+    auto fours = [](const void* at, int64_t ld) { return (uintptr_t)at % (4 * sizeof(T)) == 0 && ld % 4 == 0; };
+    p.vec = fours(c.y, c.ldo) && (!c.r || fours(c.r, c.ldr));
     p.tiles_n = pl.tiles_n();
     p.tiles_m = (int)((c.M + NT - 1) / NT);
     p.tiles = p.tiles_m * (MODE == PAIR ? (p.tiles_n + 1) / 2 : p.tiles_n);
-    p.split = split;
+    p.log2_split = log2_split;
     p.err = c.err;
     p.wait_limit = c.wait_limit > 0 ? c.wait_limit : tc::kWaitCycles;
     p.stall_mma = c.stall_mma;
-    int clusters = 0;
+    int grid = p.tiles << log2_split;
     if (MODE == PAIR) {
-        static std::atomic<int> cached{0};  // the same on every device this library is built for
-        clusters = cached.load();
-        if (!clusters) {
-            clusters = std::max(1, resident_clusters((const void*)fn, Sh::SMEM, 2));
-            cached.store(clusters);
-        }
+        static std::atomic<int> clusters{0};
+        int n = clusters.load();
+        if (!n) clusters.store(n = resident_clusters((const void*)fn, Sh::SMEM, 2));
+        grid = 2 * std::min(p.tiles, n);
     }
-    const int size = MODE == PAIR ? 2 : MODE == SPLIT ? split : 1;
+    const int size = MODE == PAIR ? 2 : 1 << log2_split;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(MODE == SPLIT ? p.tiles * split
-                                  : MODE == PAIR ? 2 * std::min(p.tiles, clusters) : std::min(p.tiles, device_sm_count())));
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(LT);
     cfg.dynamicSmemBytes = Sh::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
-    if (MODE != SINGLE) {
+    if (size > 1) {
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim.x = (unsigned)size;
         at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
@@ -751,32 +888,79 @@ bool launch(const Plan& pl, const Call& c, const Operands& op, int split, cudaSt
     return cudaLaunchKernelEx(&cfg, fn, tmx, tmw, tmg, p) == cudaSuccess;
 }
 
-// One tile width: split over K when the tiles leave half of the SMs idle, one CTA per SM otherwise.
-template <class T, int NT, int PLANES, bool GATED>
-bool run(const Plan& pl, const Call& c, const Operands& op, cudaStream_t st) {
-    const int64_t tiles = (c.M + NT - 1) / NT * pl.tiles_n();
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= device_sm_count() && pl.nkb() >= split * 4) split *= 2;
-    if (split > 1) return launch<T, NT, PLANES, GATED, SPLIT>(pl, c, op, split, st);
-    return launch<T, NT, PLANES, GATED, SINGLE>(pl, c, op, 1, st);
+bool tma_rows(const Plan& p, const Call& c) {  // the caller's 16-bit rows as they are
+    return p.planes() == 1 && (uintptr_t)c.x % 16 == 0 && c.ldx % 8 == 0;
 }
 
-template <class T, int PLANES>
-bool pick_tile(const Plan& pl, const Call& c, const Operands& op, cudaStream_t st) {
-    constexpr int WIDE = PLANES == 3 ? 128 : 256;  // widest tile whose accumulators fit in TMEM, ungated
-    auto pairs = [&](int nt) { return (c.M + nt - 1) / nt * ((pl.tiles_n() + 1) / 2); };
-    const int enough = device_sm_count() / 2;  // a tile for every pair of CTAs
-    if (pl.gated) {
-        if (pairs(WIDE / 2) >= enough && c.M > WIDE / 2) return launch<T, WIDE / 2, PLANES, true, PAIR>(pl, c, op, 1, st);
-        if (c.M <= 32) return run<T, 32, PLANES, true>(pl, c, op, st);
-        if (PLANES == 3 || c.M <= 64) return run<T, 64, PLANES, true>(pl, c, op, st);
-        return run<T, WIDE / 2, PLANES, true>(pl, c, op, st);
+struct Choice {
+    int nt = 0, mode = ONE, log2_split = 0;
+    double cycles = 0;
+};
+
+// The form and tile of a call, by an estimate of its SM cycles. Fixed parts and rates as measured
+// (clock64 stamps in the kernel): about 3000 cycles from launch to the first MMA, a K block the larger
+// of its MMAs (64 cycles each up to N = 128, N / 2 above) and its bytes at 56 a cycle, 1500 cycles for the
+// exchange in a cluster and 64 bytes a cycle stored in it, four outputs a cycle in the epilogue. Clusters of
+// 8 and 4 fit 15 and 33 times, pairs on all SMs.
+Choice choose(const Plan& p, int64_t M, bool pass) {
+    const int S = p.gated ? 2 : 1, planes = p.planes(), rowb = planes == 3 ? 64 : 128;
+    const int steps = planes == 3 ? 12 : 4, sms = device_sm_count();
+    const int widest = planes == 3 ? 128 / S : 256 / S;  // accumulators in TMEM
+    Choice best;
+    for (int nt = 32; nt <= 256; nt *= 2) {
+        const double tiles_m = (double)((M + nt - 1) / nt), mma = std::max(64, nt / 2);
+        const double rows = std::min<double>(nt, (double)M), out = rows * TR * S / 4.0;
+        if (nt <= std::min(widest, 128)) {
+            for (int l = 0; l < 4; l++) {
+                const int split = 1 << l;
+                if (l && p.nkb() < 2 * split) break;
+                const int fit = split == 8 ? 15 : split == 4 ? 33 : sms / split;
+                const double tiles = tiles_m * p.tiles_n();
+                const double waves = std::ceil(tiles / fit);
+                const double block = std::max(S * steps * mma, (S * planes * TR * rowb + planes * nt * rowb) / 56.0);
+                const double t = waves * (3000 + std::ceil((double)p.nkb() / split) * block + out / split +
+                                          (l ? 1500 + S * rows * TR * 4 / 64.0 : rows * TR * S * 4 / 256.0));
+                if (!best.nt || t < best.cycles) best = Choice{nt, ONE, l, t};
+            }
+        }
+        if (nt <= widest && nt * 4 >= widest) {
+            const double tiles = tiles_m * ((p.tiles_n() + 1) / 2);
+            const double block = std::max(S * steps * mma * 1.15, (S * planes * TR * rowb + planes * nt / 2 * rowb) / 56.0);
+            const double work = p.nkb() * block;
+            double t = 4500 + std::ceil(tiles / (sms / 2)) * std::max(work, out) + std::min(work, out);
+            if (pass) t += 5000 + (double)M * p.K * (planes == 3 ? 10 : 4) / 2500.0;
+            if (t < best.cycles) best = Choice{nt, PAIR, 0, t};
+        }
     }
-    if (pairs(WIDE) >= enough && c.M > WIDE / 2) return launch<T, WIDE, PLANES, false, PAIR>(pl, c, op, 1, st);
-    if (c.M <= 32) return run<T, 32, PLANES, false>(pl, c, op, st);
-    if (c.M <= 64) return run<T, 64, PLANES, false>(pl, c, op, st);
-    return run<T, 128, PLANES, false>(pl, c, op, st);
+    return best;
 }
+
+template <class T, int PLANES, bool GATED, bool MANUAL>
+bool run_one(const Plan& pl, const Call& c, const Operands& op, const Choice& ch, cudaStream_t st) {
+    if (ch.nt == 32) return launch<T, 32, PLANES, GATED, ONE, MANUAL>(pl, c, op, ch.log2_split, st);
+    if (ch.nt == 64) return launch<T, 64, PLANES, GATED, ONE, MANUAL>(pl, c, op, ch.log2_split, st);
+    return launch<T, PLANES == 3 && GATED ? 64 : 128, PLANES, GATED, ONE, MANUAL>(pl, c, op, ch.log2_split, st);
+}
+template <class T, int PLANES, bool GATED>
+bool run_pair(const Plan& pl, const Call& c, const Operands& op, const Choice& ch, cudaStream_t st) {
+    constexpr int W = (PLANES == 3 ? 128 : 256) / (GATED ? 2 : 1);
+    if (ch.nt == W) return launch<T, W, PLANES, GATED, PAIR, false>(pl, c, op, 0, st);
+    if (ch.nt == W / 2) return launch<T, W / 2, PLANES, GATED, PAIR, false>(pl, c, op, 0, st);
+    return launch<T, W / 4 < 32 ? 32 : W / 4, PLANES, GATED, PAIR, false>(pl, c, op, 0, st);
+}
+template <class T, int PLANES, bool GATED>
+bool run(const Plan& pl, const Call& c, const Operands& op, const Choice& ch, cudaStream_t st) {
+    if (ch.mode == PAIR) return run_pair<T, PLANES, GATED>(pl, c, op, ch, st);
+    if constexpr (PLANES == 3) return run_one<T, PLANES, GATED, true>(pl, c, op, ch, st);
+    else return tma_rows(pl, c) ? run_one<T, PLANES, GATED, false>(pl, c, op, ch, st) : run_one<T, PLANES, GATED, true>(pl, c, op, ch, st);
+}
+template <class T, int PLANES>
+bool run(const Plan& pl, const Call& c, const Operands& op, const Choice& ch, cudaStream_t st) {
+    return pl.gated ? run<T, PLANES, true>(pl, c, op, ch, st) : run<T, PLANES, false>(pl, c, op, ch, st);
+}
+
+unsigned grid_for(int64_t items) { return (unsigned)std::min<int64_t>((items + 255) / 256, (int64_t)device_sm_count() * 16); }
+int kp_of(const Plan& p) { return p.planes() == 3 ? p.nkb() * 32 : (p.K + 7) / 8 * 8; }
 }  // namespace
 
 void layout(const Plan& p, const void* w, uint8_t* tiles, float* rows, cudaStream_t st) {
@@ -790,28 +974,27 @@ void layout(const Plan& p, const void* w, uint8_t* tiles, float* rows, cudaStrea
 }
 
 size_t tc_workspace(const Plan& p, const Call& c) {
-    if (tma_rows(p, c)) return 0;
+    if (tma_rows(p, c) || choose(p, c.M, true).mode == ONE) return 0;
     return (size_t)p.planes() * c.M * kp_of(p) * 2;
 }
 
 int tc(const Plan& p, const Call& c, void* ws, cudaStream_t st) {
-    const void* x = c.x;
-    int64_t ldx = c.ldx;
+    const bool direct = tma_rows(p, c);
+    const Choice ch = choose(p, c.M, !direct);
+    Operands op{c.x, c.ldx, p.K};
     int n = 0;
-    if (!tma_rows(p, c)) {
+    if (!direct && ch.mode == PAIR) {
         const int kp = kp_of(p);
         const unsigned grid = grid_for(c.M * (kp / 8));
         if (p.planes() == 3) k_split_x<<<grid, 256, 0, st>>>((const float*)c.x, c.ldx, c.M, p.K, kp, (uint16_t*)ws);
         else k_pack_x<<<grid, 256, 0, st>>>((const uint16_t*)c.x, c.ldx, c.M, p.K, kp, (uint16_t*)ws);
-        x = ws;
-        ldx = kp;
+        op = Operands{ws, kp, kp};
         n++;
     }
-    const Operands op{x, ldx, x == c.x ? p.K : kp_of(p)};
     bool ok;
-    if (p.dtype == DT_F32) ok = pick_tile<float, 3>(p, c, op, st);
-    else if (p.dtype == DT_F16) ok = pick_tile<__half, 1>(p, c, op, st);
-    else ok = pick_tile<__nv_bfloat16, 1>(p, c, op, st);
+    if (p.dtype == DT_F32) ok = run<float, 3>(p, c, op, ch, st);
+    else if (p.dtype == DT_F16) ok = run<__half, 1>(p, c, op, ch, st);
+    else ok = run<__nv_bfloat16, 1>(p, c, op, ch, st);
     return ok ? n + 1 : -1;
 }
 
