@@ -363,21 +363,23 @@ struct Chunk<3> {
 // stage's full barrier counts its groups. LW is such that a warp has a group in at least every ST-th block:
 // when it waits for block n's stage it then knows block n - 2 ST consumed (it has waited for a later one), so
 // the parity it waits for cannot be an older phase's.
-template <class T, int NT, int PLANES, bool GATED, int MODE>
-__device__ bool load_rows(const TcParams& p, int m0, int kb0, int kb1, int w, int lane, uint32_t sbase, uint32_t full0,
-                          uint32_t empty0, long long limit) {
-    using Sh = Shape<NT, PLANES, GATED, MODE>;
-    constexpr int PER = Sh::ROWB / 16, ST = Sh::STAGES;  // chunks of a row in a block
-    constexpr int LW = Sh::GROUPS_X * ST < EPI ? Sh::GROUPS_X * ST : EPI;
+template <class Sh, int PLANES>
+struct RowLoader {
+    static constexpr int PER = Sh::ROWB / 16, ST = Sh::STAGES;  // chunks of a row in a block
+    static constexpr int LW = Sh::GROUPS_X * ST < EPI ? Sh::GROUPS_X * ST : EPI;
     static_assert(Sh::GROUPS_X >= EPI || LW % Sh::GROUPS_X == 0, "a warp's groups lie LW / GROUPS_X blocks apart");
-    if (w >= LW) return true;
-    const int groups = (kb1 - kb0) * Sh::GROUPS_X;
-    Chunk<PLANES> buf[2];
-    auto fetch = [&](Chunk<PLANES>& c, int g) {
+    const TcParams& p;
+    int m0, kb0, lane, next;  // next: the warp's next group, counted from block kb0
+    uint32_t sbase, full0, empty0;
+
+    __device__ RowLoader(const TcParams& params, int m, int kb, int warp, int ln, uint32_t base, uint32_t full, uint32_t empty)
+        : p(params), m0(m), kb0(kb), lane(ln), next(warp < LW ? warp : 1 << 30), sbase(base), full0(full), empty0(empty) {}
+
+    __device__ __forceinline__ void fetch(Chunk<PLANES>& c, int g, int groups) const {
         const int i = (g % Sh::GROUPS_X) * 32 + lane;
         if (g < groups) c.load(p, m0 + i / PER, (kb0 + g / Sh::GROUPS_X) * (Sh::ROWB / 2) + i % PER * 8);
-    };
-    auto put = [&](const Chunk<PLANES>& c, int g) {
+    }
+    __device__ __forceinline__ bool put(const Chunk<PLANES>& c, int g, long long limit) const {
         const int i = (g % Sh::GROUPS_X) * 32 + lane, n = g / Sh::GROUPS_X, s = n % ST;
         if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((uint32_t)(n / ST) & 1u) ^ 1u, limit))) return false;
         c.store(sbase + s * Sh::STAGE + Sh::S * Sh::WB, Sh::XR, i / PER, i % PER);
@@ -385,17 +387,24 @@ __device__ bool load_rows(const TcParams& p, int m0, int kb0, int kb1, int w, in
         __syncwarp();
         if (lane == 0) mbar_arrive(full0 + 8 * s);
         return true;
-    };
-    fetch(buf[0], w);
-    for (int g = w; g < groups; g += 2 * LW) {
-        fetch(buf[1], g + LW);
-        if (!put(buf[0], g)) return false;
-        if (g + LW >= groups) break;
-        fetch(buf[0], g + 2 * LW);
-        if (!put(buf[1], g + LW)) return false;
     }
-    return true;
-}
+    // Fills this warp's groups of the first `blocks` K blocks that it has not filled yet.
+    __device__ bool fill(int blocks, long long limit) {
+        const int groups = blocks * Sh::GROUPS_X;
+        Chunk<PLANES> buf[2];
+        fetch(buf[0], next, groups);
+        while (next < groups) {
+            fetch(buf[1], next + LW, groups);
+            if (!put(buf[0], next, limit)) return false;
+            next += LW;
+            if (next >= groups) break;
+            fetch(buf[0], next + LW, groups);
+            if (!put(buf[1], next, limit)) return false;
+            next += LW;
+        }
+        return true;
+    }
+};
 
 template <class T, int NT, int PLANES, bool GATED, int MODE, bool MANUAL>
 __global__ void __launch_bounds__(LT, 1)
@@ -455,7 +464,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     const int tstep = MODE == ONE ? p.tiles : (int)gridDim.x / CG;
     const int kb0 = MODE == ONE ? (int)(((int64_t)p.nkb * rank) >> p.log2_split) : 0;
     const int kb1 = MODE == ONE ? (int)(((int64_t)p.nkb * (rank + 1)) >> p.log2_split) : p.nkb;
-    constexpr int CH = PLANES == 3 ? CHUNK : 1 << 30;
+    constexpr int CH = PLANES == 3 ? CHUNK : 1 << 28;
 
     if (warp == 0) {
         if (lane == 0) {  // producer, running ahead across tiles
@@ -578,8 +587,10 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
             const int n0 = (MODE == PAIR ? 2 * tn + rank : tn) * TR;
             Columns<T, GATED> out;
             out.begin(p, n0 + (tid & 15) * 4);
-            if (MANUAL && !load_rows<T, NT, PLANES, GATED, MODE>(p, tm * NT, kb0, kb1, warp - 2, lane, sbase, full0, empty0, limit))
-                s_fail = 1;  // the wait below runs out too
+            // The rows of two accumulator chunks ahead of the one being read: the MMAs of chunk i wait for the
+            // sums of chunk i - 2 to be read, so rows past chunk i + 1 must not be waited for before that.
+            RowLoader<Sh, PLANES> rows(p, tm * NT, kb0, warp - 2, lane, sbase, full0, empty0);
+            if (MANUAL && !rows.fill(kb1 - kb0 < 2 * CH ? kb1 - kb0 : 2 * CH, limit)) s_fail = 1;  // the wait below runs out too
             float acc[PLANES == 3 ? S : 1][PLANES == 3 ? HC : 1];  // f32: the promoted sums
             bool ok = true;
             int chunks = 0;
@@ -604,6 +615,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                             for (int j = 0; j < SLAB; j++) acc[v][c + j] = chunks ? acc[v][c + j] + (a[j] + k[j]) : a[j] + k[j];
                         }
                     release(buf);
+                    if (MANUAL && !rows.fill(kb1 - c0 < 3 * CH ? kb1 - kb0 : c0 - kb0 + 3 * CH, limit)) s_fail = 1;
                 }
             }
             const int buf = (use - 1) & 1;

@@ -153,6 +153,15 @@ def test_persistent_tiles(ctx, dtype, M, K, N):
     Case(ctx, dtype, M, K, N, act="silu", gated=True).check()
 
 
+@pytest.mark.parametrize("dtype,M,K,N,gated,pad", [("f32", 20, 2048, 19000, False, 0), ("f32", 30, 1111, 19000, True, 1),
+                                                   ("f32", 60, 1500, 19000, False, 0), ("f16", 31, 3001, 19000, False, 3),
+                                                   ("bf16", 64, 2500, 19000, True, 1), ("bf16", 100, 4096, 18000, False, 0)])
+def test_long_sums_of_one_tile(ctx, dtype, M, K, N, gated, pad):
+    """So many weight tiles that none is split over K: one CTA goes through every K block, its stages many
+    times over, and in f32 through many promotions, with its rows loaded by TMA and by the epilogue's warps."""
+    Case(ctx, dtype, M, K, N, act="silu" if gated else "none", gated=gated, pad=pad).check()
+
+
 @pytest.mark.parametrize("M,K,N", [(64, 768, 512), (300, 2048, 640), (1000, 4096, 768), (20, 4096, 256), (4, 4096, 512)])
 def test_f32_is_as_exact_as_fp32(ctx, M, K, N):
     c = Case(ctx, "f32", M, K, N)
