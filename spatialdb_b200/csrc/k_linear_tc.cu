@@ -269,21 +269,47 @@ __device__ __forceinline__ void tile_at(const TcParams& p, int tiles_n, int t, i
     tn = i / width;
 }
 
-__device__ __forceinline__ uint16_t bf16_cut(float v) { return (uint16_t)(__float_as_uint(v) >> 16); }
-
-// The three bf16 parts of an fp32 value, each the leading eight significant bits of what is left
-// (truncated, so no part overflows): their sum is the value exactly. A value that is not finite keeps
-// itself in the first part (a NaN stays one) and zeros in the others.
-__device__ __forceinline__ void split3(float v, uint16_t (&o)[3]) {
-    o[0] = bf16_cut(v);
-    o[1] = o[2] = 0;
-    if (!isfinite(v)) {
-        if (isnan(v)) o[0] |= 0x40;
-        return;
+// The three bf16 parts of eight fp32 values, each the leading eight significant bits of what is left (cut
+// off, so no part overflows): their sum is the value exactly. Of a value that is not finite the first part
+// keeps it (a NaN stays one) and the others are zero.
+__device__ __forceinline__ void split3(const float (&f)[8], uint4 (&part)[3]) {
+    float r[8], q[8];
+    uint32_t w[3][4];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        r[j] = f[j] - __uint_as_float(__float_as_uint(f[j]) & 0xFFFF0000u);
+        q[j] = r[j] - __uint_as_float(__float_as_uint(r[j]) & 0xFFFF0000u);
     }
-    const float r1 = v - __uint_as_float((uint32_t)o[0] << 16);
-    o[1] = bf16_cut(r1);
-    o[2] = bf16_cut(r1 - __uint_as_float((uint32_t)o[1] << 16));
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        w[0][j] = __byte_perm(__float_as_uint(f[2 * j]), __float_as_uint(f[2 * j + 1]), 0x7632);
+        w[1][j] = __byte_perm(__float_as_uint(r[2 * j]), __float_as_uint(r[2 * j + 1]), 0x7632);
+        w[2][j] = __byte_perm(__float_as_uint(q[2 * j]), __float_as_uint(q[2 * j + 1]), 0x7632);
+    }
+    const float sum = ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+    if (isnan(sum)) {  // inf - inf and NaN - NaN: some value is not finite
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (isfinite(f[j])) continue;
+            const uint32_t keep = j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+            if (isnan(f[j])) w[0][j / 2] |= 0x00400040u & ~keep;
+            w[1][j / 2] &= keep;
+            w[2][j / 2] &= keep;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 3; i++) part[i] = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+}
+
+// Shared-memory matrix descriptors, K-major: the operand's start goes into the low word (in 16-byte units),
+// the rest is constant: rows of 128 bytes in groups of 1 KB with the 128-byte swizzle, or of 64 bytes in groups of
+// 512 with the 64-byte one.
+template <int ROWB>
+__device__ __forceinline__ uint64_t operand(uint32_t start) {
+    constexpr uint32_t HI = (uint32_t)(8 * ROWB >> 4) | 1u << 14 | (ROWB == 128 ? 2u : 4u) << 29;  // group stride, version, swizzle
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(start), "n"(HI));
+    return d;
 }
 
 // Eight values of a row from column k, zeros past K: as few and wide loads as the address allows.
@@ -341,19 +367,12 @@ struct Chunk<3> {
     }
     // The three parts' planes of 64-byte rows, chunks XORed with (r / 2) % 4.
     __device__ __forceinline__ void store(uint32_t area, int rows, int r, int c) const {
-        uint16_t e[3][8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            uint16_t o[3];
-            split3(f[j], o);
-#pragma unroll
-            for (int q = 0; q < 3; q++) e[q][j] = o[q];
-        }
+        uint4 w[3];
+        split3(f, w);
 #pragma unroll
         for (int q = 0; q < 3; q++) {
             const uint32_t at = area + q * rows * 64 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-            const uint4 w = *(const uint4*)e[q];
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[q].x), "r"(w[q].y), "r"(w[q].z), "r"(w[q].w) : "memory");
         }
     }
 };
@@ -524,19 +543,20 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                     for (int kb = c0; kb < c1; kb++) {
                         if (p.stall_mma || !mbar_wait(full0 + 8 * s, ph, limit)) { ok = false; break; }
                         fence_after();
-                        const uint32_t w = sbase + s * Sh::STAGE, x = w + S * Sh::WB;
+                        // operand starts in 16-byte units (the leading byte offset's 1 is ignored for these layouts)
+                        const uint32_t w0 = ((sbase + s * Sh::STAGE) >> 4) | 1u << 16, x0 = w0 + (S * Sh::WB >> 4);
 #pragma unroll
                         for (int kk = 0; kk < ROWB / 32; kk++) {
                             const uint32_t first = kb == c0 && kk == 0 ? 0u : 1u;
 #pragma unroll
                             for (int v = 0; v < S; v++) {
+                                const uint32_t w = w0 + (v * Sh::WB >> 4) + 2 * kk, x = x0 + 2 * kk;
                                 if (PLANES == 1) {
-                                    umma_f16<CG>(d + v * NT, sw128_desc(w + v * Sh::WB + kk * 32), sw128_desc(x + kk * 32), idesc, first);
+                                    umma_f16<CG>(d + v * NT, operand<ROWB>(w), operand<ROWB>(x), idesc, first);
                                 } else {
-                                    const uint32_t wb = w + v * Sh::WB + kk * 32, xb = x + kk * 32;
-                                    constexpr int WP = TR * ROWB, XP = Sh::XR * ROWB;
-                                    const uint64_t w1 = sw64_desc(wb), w2 = sw64_desc(wb + WP), w3 = sw64_desc(wb + 2 * WP);
-                                    const uint64_t x1 = sw64_desc(xb), x2 = sw64_desc(xb + XP), x3 = sw64_desc(xb + 2 * XP);
+                                    constexpr uint32_t WP = TR * ROWB >> 4, XP = Sh::XR * ROWB >> 4;
+                                    const uint64_t w1 = operand<ROWB>(w), w2 = operand<ROWB>(w + WP), w3 = operand<ROWB>(w + 2 * WP);
+                                    const uint64_t x1 = operand<ROWB>(x), x2 = operand<ROWB>(x + XP), x3 = operand<ROWB>(x + 2 * XP);
                                     const uint32_t da = d + 2 * v * NT, db = da + NT;
                                     umma_f16<CG>(da, w1, x1, idesc, first);
                                     umma_f16<CG>(db, w1, x2, idesc, first);
@@ -768,17 +788,14 @@ __global__ void k_tiles32(const float* __restrict__ w, int N, int K, int nkb, in
         const int64_t blk = i >> 9;
         const int64_t n = blk / nkb * TR + row;
         const int k = (int)(blk % nkb) * 32 + c * 8;
-        uint16_t e[3][8];
+        float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            uint16_t o[3];
-            split3(n < N && k + j < K ? w[n * K + k + j] : 0.0f, o);
-#pragma unroll
-            for (int q = 0; q < 3; q++) e[q][j] = o[q];
-        }
+        for (int j = 0; j < 8; j++) f[j] = n < N && k + j < K ? w[n * K + k + j] : 0.0f;
+        uint4 part[3];
+        split3(f, part);
 #pragma unroll
         for (int q = 0; q < 3; q++)
-            *(uint4*)(out + blk * (3 * TR * 64) + q * (TR * 64) + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)) = *(const uint4*)e[q];
+            *(uint4*)(out + blk * (3 * TR * 64) + q * (TR * 64) + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)) = part[q];
     }
 }
 
@@ -796,16 +813,10 @@ __global__ void k_split_x(const float* __restrict__ x, int64_t ldx, int64_t M, i
         const int k = (int)(i % (kp / 8)) * 8;
         float f[8];
         row8(x + m * ldx, k, K, f);
-        uint16_t e[3][8];
+        uint4 part[3];
+        split3(f, part);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            uint16_t o[3];
-            split3(f[j], o);
-#pragma unroll
-            for (int q = 0; q < 3; q++) e[q][j] = o[q];
-        }
-#pragma unroll
-        for (int q = 0; q < 3; q++) *(uint4*)(out + (q * M + m) * kp + k) = *(const uint4*)e[q];
+        for (int q = 0; q < 3; q++) *(uint4*)(out + (q * M + m) * kp + k) = part[q];
     }
 }
 
@@ -929,7 +940,8 @@ Choice choose(const Plan& p, int64_t M, bool pass) {
                 const int fit = split == 8 ? 15 : split == 4 ? 33 : sms / split;
                 const double tiles = tiles_m * p.tiles_n();
                 const double waves = std::ceil(tiles / fit);
-                const double block = std::max(S * steps * mma, (S * planes * TR * rowb + planes * nt * rowb) / 56.0);
+                double block = std::max(S * steps * mma, (S * planes * TR * rowb + planes * nt * rowb) / 56.0);
+                if (pass) block = std::max(block, planes == 3 ? 1100.0 + 6.0 * nt : 500.0 + nt);
                 const double t = waves * (3000 + std::ceil((double)p.nkb() / split) * block + out / split +
                                           (l ? 1500 + S * rows * TR * 4 / 64.0 : rows * TR * S * 4 / 256.0));
                 if (!best.nt || t < best.cycles) best = Choice{nt, ONE, l, t};
@@ -940,7 +952,7 @@ Choice choose(const Plan& p, int64_t M, bool pass) {
             const double block = std::max(S * steps * mma * 1.15, (S * planes * TR * rowb + planes * nt / 2 * rowb) / 56.0);
             const double work = p.nkb() * block;
             double t = 4500 + std::ceil(tiles / (sms / 2)) * std::max(work, out) + std::min(work, out);
-            if (pass) t += 5000 + (double)M * p.K * (planes == 3 ? 10 : 4) / 2500.0;
+            if (pass) t += 3500 + (double)M * p.K * (planes == 3 ? 10 : 4) / 3000.0;
             if (t < best.cycles) best = Choice{nt, PAIR, 0, t};
         }
     }
