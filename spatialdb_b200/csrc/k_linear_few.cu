@@ -1,14 +1,17 @@
 // k_linear_few.cu -- the linear operator for few rows (decoded tokens): the weights are read once and
 // nothing else matters, so the kernels are built around the weight stream.
 //
-// 16-bit, up to 16 rows: one block per 16 weight rows, its eight warps taking 64-wide K blocks in turn.
-// In the tiled layout 16 rows of a K block are 2 KB in a row; a lane loads 16-byte chunks t and t + 4 of
-// rows g and g + 8 (g = lane / 4, t = lane % 4). A chunk's eight values feed two m16n8k16 products whose
-// K order is permuted alike on both sides (a sum does not care), so weights go from memory to the
-// matrix instruction without shared memory or shuffles; x comes from cache in the same order. The
-// tensor pipe is idle most of the time: what counts is the bytes in flight.
+// 16-bit, up to 16 rows: one block per 16 weight rows, its eight warps taking 64-wide K blocks in turn, two
+// at a time (everything they need is asked for before any of it is used; four at a time take the registers
+// of half the blocks: 18.3 against 16.5 us below). In the tiled layout 16 rows of a K block are 2 KB in a
+// row; a lane loads 16-byte chunks t and t + 4 of rows g and g + 8 (g = lane / 4, t = lane % 4). A chunk's
+// eight values feed two m16n8k16 products whose K order is permuted alike on both sides (a sum does not
+// care), so weights go from memory to the matrix instruction without shared memory or shuffles; x comes from
+// cache in the same order. The tensor pipe is idle most of the time: what counts is the bytes in flight.
+// bf16 1 x 4096 x 11008: 16.5 us, 5455 GB/s; f16 8 x 4096 x 4096: 8.5 us; bf16 1 x 2048 x 16384 gated: 21.8 us,
+// 6148 GB/s.
 // f32, up to 8 rows: one block per 8 weight rows (4 + 4 when gated), four consecutive K values a lane,
-// fp32 FMAs.
+// fp32 FMAs. 1 x 4096 x 11008: 29.7 us, 6076 GB/s.
 // Both join the warps' partial sums in shared memory in a fixed order and apply the epilogue there.
 #include <algorithm>
 #include <cstdint>
@@ -81,7 +84,7 @@ __device__ __forceinline__ void finish(const FewParams& p, int m, int n, float a
 // MT: tiles of 8 activation rows. VEC: x rows start on 16-byte boundaries.
 template <class T, int MT, bool GATED, bool VEC>
 __global__ void __launch_bounds__(FT) k_few16(FewParams p) {
-    constexpr int S = GATED ? 2 : 1, U = 2;  // K blocks a warp has in flight
+    constexpr int S = GATED ? 2 : 1, U = GATED ? 1 : 2;  // K blocks a warp has in flight
     __shared__ float red[WARPS][S][MT][8][16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int grp = blockIdx.x, n0 = grp * 16;
@@ -96,38 +99,37 @@ __global__ void __launch_bounds__(FT) k_few16(FewParams p) {
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[s][i][j] = 0.0f;
     for (int kb0 = warp; kb0 < p.nkb; kb0 += WARPS * U) {
-        uint4 w[U][S][4];
+        // everything the U blocks need is asked for before any of it is used
+        uint4 w[U][S][4], x[U][MT][2];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int kb = kb0 + u * WARPS;
-            if (kb >= p.nkb) break;
+            const bool live = kb < p.nkb;
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                const uint8_t* q = src[s] + (int64_t)kb * TR * 128;
+                const uint8_t* q = src[s] + (int64_t)(live ? kb : kb0) * TR * 128;  // past the end: a block once more, times zeros
                 w[u][s][0] = __ldg((const uint4*)(q + off));
                 w[u][s][1] = __ldg((const uint4*)(q + off + 1024));
                 w[u][s][2] = __ldg((const uint4*)(q + (off ^ 64)));
                 w[u][s][3] = __ldg((const uint4*)(q + (off ^ 64) + 1024));
             }
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) x[u][i][c] = load_x8<T, VEC>(p, live ? g + 8 * i : p.M, kb * 64 + c * 32 + t * 8);
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int kb = kb0 + u * WARPS;
-            if (kb >= p.nkb) break;
+        for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const uint4 x = load_x8<T, VEC>(p, g + 8 * i, kb * 64 + c * 32 + t * 8);
+                for (int c = 0; c < 2; c++)
 #pragma unroll
                     for (int s = 0; s < S; s++) {
-                        const uint4 lo = w[u][s][2 * c], hi = w[u][s][2 * c + 1];
-                        mma16816<T>(acc[s][i], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
-                        mma16816<T>(acc[s][i], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+                        const uint4 lo = w[u][s][2 * c], hi = w[u][s][2 * c + 1], v = x[u][i][c];
+                        mma16816<T>(acc[s][i], lo.x, hi.x, lo.y, hi.y, v.x, v.y);
+                        mma16816<T>(acc[s][i], lo.z, hi.z, lo.w, hi.w, v.z, v.w);
                     }
-                }
-            }
-        }
     }
 #pragma unroll
     for (int s = 0; s < S; s++)
@@ -165,7 +167,7 @@ __device__ __forceinline__ float4 load_x4(const FewParams& p, int m, int64_t k) 
 
 // MB: activation rows (1, 2, 4, 8).
 template <int MB, bool GATED, bool VEC>
-__global__ void __launch_bounds__(FT) k_few32(FewParams p) {
+__global__ void __launch_bounds__(FT, MB >= 4 ? 2 : 3) k_few32(FewParams p) {
     constexpr int S = GATED ? 2 : 1, R = 8 / S, NV = 8 * MB;  // weight rows a block, sums a lane
     __shared__ float red[WARPS][NV];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -242,7 +244,13 @@ void launch32(const FewParams& p, cudaStream_t st) {
 }
 }  // namespace
 
-bool few_supported(const Plan& p, int64_t M) { return M <= (p.dtype == DT_F32 ? 8 : 16); }
+// f32 past 4 rows: the sums leave few registers for loads, and the tensor-core form, which reads six bytes a
+// weight instead of four, catches up from about 8 million weights on (8 rows, 4096 x 4096: 31.0 us here,
+// 25.9 there; 768 x 2304: 4.2 and 9.1).
+bool few_supported(const Plan& p, int64_t M) {
+    if (p.dtype != DT_F32) return M <= 16;
+    return M <= 4 || (M <= 8 && (int64_t)p.N * p.K * (p.gated ? 2 : 1) <= (8 << 20));
+}
 
 int few(const Plan& pl, const Call& c, cudaStream_t st) {
     FewParams p;
