@@ -223,7 +223,7 @@ slx_status slx_attention(slx_ctx* ctx, const int64_t* q, const int64_t* k, const
  * own type. d_gate NULL: no gate. Sums and the epilogue are fp32, rounded once to dtype.
  * An F32 product of more than 8 rows runs on the tensor cores from three bf16 parts of every value: a
  * finite result is as exact as an fp32 sum, an infinite x or w gives an infinity or a NaN.
- * slx_linear_device: x [M][K], residual (nullable) and y [M][N] with row strides in elements, at least the
+ * slx_linear_device (device pointers): x [M][K], residual (nullable) and y [M][N] with row strides in elements, at least the
  * row's width; y may be the residual's buffer (same stride) and must not overlap x otherwise. Any M >= 0.
  * Results do not change from call to call. A bounded wait that gave up is reported by slx_ctx_status
  * (SLX_ETIMEOUT). info: dtype, N, K, act, gated, device bytes held. */
@@ -233,8 +233,16 @@ slx_status slx_linear_prepare(slx_ctx* ctx, int dtype, const uint8_t* d_w, int64
                               const float* d_gate_bias, slx_linear** out);
 slx_status slx_linear_free(slx_linear* l);
 slx_status slx_linear_info(slx_linear* l, int64_t* info, int n);
-slx_status slx_linear_device(slx_linear* l, const void* d_x, int64_t ldx, int64_t M, const void* d_residual, int64_t ldr,
-                             void* d_y, int64_t ldy, void* stream);
+typedef struct slx_linear_args { /* one call's arguments, in memory: a foreign call then passes two pointers */
+    const void* x;
+    int64_t ldx, M;
+    const void* residual;
+    int64_t ldr;
+    void* y;
+    int64_t ldy;
+    void* stream;
+} slx_linear_args;
+slx_status slx_linear_device(slx_linear* l, const slx_linear_args* args);
 
 /* Norms of the queries and keys for each head and the rotary positions, in one pass. For a head row x:
  * u = x / sqrt(mean(x^2) + eps) * w (u = x without a weight), then (u_p, u_{p+h}) for p < h = rot_dim / 2 is
@@ -247,7 +255,7 @@ slx_status slx_linear_device(slx_linear* l, const void* d_x, int64_t ldx, int64_
  * int64 for Q30; NULL: that side is rotated only; complete before the call, copied). rot_dim <= head_dim (Q30: equal, eps 0).
  * slx_qk_norm_rope_device: q [M][heads * head_dim] to qo, k [M][kv_heads * head_dim] to ko, row strides in
  * elements, at least the row's width; an output may be its input (same stride) and must not overlap the
- * inputs otherwise. Row m stands at d_pos[m], or at m % T when d_pos is NULL. A position of -1 leaves the
+ * inputs otherwise. Row m stands at pos[m], or at m % T when pos is NULL. A position of -1 leaves the
  * row's outputs as they were; another one outside the table does too and is reported by slx_ctx_status
  * (SLX_ERANGE). heads or kv_heads may be 0 (its pointers are not read). A table may be freed before the
  * layers that use it. */
@@ -258,9 +266,19 @@ slx_status slx_rope_free(slx_rope* r);
 slx_status slx_qk_norm_prepare(slx_rope* r, int dtype, int heads, int kv_heads, int head_dim, const void* d_wq,
                                const void* d_wk, float eps, slx_qk_norm** out);
 slx_status slx_qk_norm_free(slx_qk_norm* h);
-slx_status slx_qk_norm_rope_device(slx_qk_norm* h, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, int64_t M,
-                                   int64_t T, const int32_t* d_pos, void* d_qo, int64_t ldqo, void* d_ko, int64_t ldko,
-                                   void* stream);
+typedef struct slx_qk_args {
+    const void* q;
+    int64_t ldq;
+    const void* k;
+    int64_t ldk, M, T;
+    const int32_t* pos;
+    void* qo;
+    int64_t ldqo;
+    void* ko;
+    int64_t ldko;
+    void* stream;
+} slx_qk_args;
+slx_status slx_qk_norm_rope_device(slx_qk_norm* h, const slx_qk_args* args);
 
 /* ---- lattice k-NN search ------------------------------------------------------------------------ */
 /* The embed+search path: EmbeddingLattice<TPayload>(occupants) + QueryKNearestL2(center, k)

@@ -18,6 +18,7 @@ All work runs in the CUDA library; nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes
+import struct
 import weakref
 
 import numpy as np
@@ -192,6 +193,10 @@ class PreparedWeight:
             pass
 
 
+_LINEAR_ARGS = struct.Struct("=QqqQqQqQ").pack       # slx_linear_args
+_QK_ARGS = struct.Struct("=QqQqqqQQqQqQ").pack       # slx_qk_args
+
+
 class Linear:
     """Float matrix product with its epilogue (slx_linear_prepare): y = act(x . w^T + bias) + residual, or
     with gate weights act(x . gate^T + gate_bias) * (x . w^T + bias) + residual. `dtype` (DTYPE_F32, DTYPE_F16,
@@ -217,7 +222,7 @@ class Linear:
                      stream: int = 0):
         """Queue y[M][N] for x[M][K] on device buffers (raw pointers; row strides in elements, 0: the row's
         width). y may be the residual's buffer."""
-        st = self._call(self._h, d_x, ldx or self.K, M, d_residual or None, ldr or self.N, d_y, ldo or self.N, stream or None)
+        st = self._call(self._h, _LINEAR_ARGS(d_x, ldx or self.K, M, d_residual, ldr or self.N, d_y, ldo or self.N, stream))
         if st:
             self.ctx.check(st)
 
@@ -282,8 +287,8 @@ class QkNormRope:
         """Queue M rows (raw device pointers; row strides in elements, 0: the row's width): q [M][heads][head_dim]
         to qo, k [M][kv_heads][head_dim] to ko (an output may be its input). Row m stands at the int32 position
         d_pos[m] (-1: left alone), or without d_pos at m % T (T 0: one sequence of M rows)."""
-        st = self._call(self._h, d_q or None, ldq or self._q, d_k or None, ldk or self._k, M, T or M, d_pos or None,
-                        d_qo or None, ldqo or self._q, d_ko or None, ldko or self._k, stream or None)
+        st = self._call(self._h, _QK_ARGS(d_q, ldq or self._q, d_k, ldk or self._k, M, T or M, d_pos, d_qo, ldqo or self._q,
+                                          d_ko, ldko or self._k, stream))
         if st:
             self.ctx.check(st)
 

@@ -56,12 +56,12 @@ SIGNATURES = {
     "slx_linear_prepare": (i, [VP, i, VP, i64, i, i, i, VP, i, VP, i64, VP, ctypes.POINTER(VP)]),
     "slx_linear_free": (i, [VP]),
     "slx_linear_info": (i, [VP, I64P, i]),
-    "slx_linear_device": (i, [VP, VP, i64, i64, VP, i64, VP, i64, VP]),
+    "slx_linear_device": (i, [VP, ctypes.c_char_p]),  # the packed slx_linear_args
     "slx_rope_create": (i, [VP, i, i, f32, i, ctypes.POINTER(VP)]),
     "slx_rope_free": (i, [VP]),
     "slx_qk_norm_prepare": (i, [VP, i, i, i, i, VP, VP, f32, ctypes.POINTER(VP)]),
     "slx_qk_norm_free": (i, [VP]),
-    "slx_qk_norm_rope_device": (i, [VP, VP, i64, VP, i64, i64, i64, VP, VP, i64, VP, i64, VP]),
+    "slx_qk_norm_rope_device": (i, [VP, ctypes.c_char_p]),  # the packed slx_qk_args
     "slx_lattice_build": (i, [VP, F32P, i64, i, f32, i64, i64, ctypes.POINTER(VP)]),
     "slx_lattice_build_device": (i, [VP, VP, i64, i, f32, i64, i64, VP, ctypes.POINTER(VP)]),
     "slx_lattice_free": (i, [VP]),

@@ -564,7 +564,7 @@ bool encode_rows_planes(void* map128, const void* base, int64_t width, int64_t r
         return false;
     if (((uintptr_t)base & 15) != 0 || (ld * 2) % 16 != 0) return false;
     cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)rows, (cuuint64_t)planes};
-    cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)(ld * rows * 2)};
+    cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)((planes > 1 ? rows : 1) * ld * 2)};
     cuuint32_t box[3] = {(cuuint32_t)box_k, (cuuint32_t)box_rows, (cuuint32_t)planes};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn((CUtensorMap*)map128, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box,

@@ -915,50 +915,6 @@ bool tma_rows(const Plan& p, const Call& c) {  // the caller's 16-bit rows as th
     return p.planes() == 1 && (uintptr_t)c.x % 16 == 0 && c.ldx % 8 == 0;
 }
 
-struct Choice {
-    int nt = 0, mode = ONE, log2_split = 0;
-    double cycles = 0;
-};
-
-// The form and tile of a call, by an estimate of its SM cycles. Fixed parts and rates as measured
-// (clock64 stamps in the kernel): about 3000 cycles from launch to the first MMA, a K block the larger
-// of its MMAs (64 cycles each up to N = 128, N / 2 above) and its bytes at 56 a cycle, 1500 cycles for the
-// exchange in a cluster and 64 bytes a cycle stored in it, four outputs a cycle in the epilogue. Clusters of
-// 8 and 4 fit 15 and 33 times, pairs on all SMs.
-Choice choose(const Plan& p, int64_t M, bool pass) {
-    const int S = p.gated ? 2 : 1, planes = p.planes(), rowb = planes == 3 ? 64 : 128;
-    const int steps = planes == 3 ? 12 : 4, sms = device_sm_count();
-    const int widest = planes == 3 ? 128 / S : 256 / S;  // accumulators in TMEM
-    Choice best;
-    for (int nt = 32; nt <= 256; nt *= 2) {
-        const double tiles_m = (double)((M + nt - 1) / nt), mma = std::max(64, nt / 2);
-        const double rows = std::min<double>(nt, (double)M), out = rows * TR * S / 4.0;
-        if (nt <= std::min(widest, 128)) {
-            for (int l = 0; l < 4; l++) {
-                const int split = 1 << l;
-                if (l && p.nkb() < 2 * split) break;
-                const int fit = split == 8 ? 15 : split == 4 ? 33 : sms / split;
-                const double tiles = tiles_m * p.tiles_n();
-                const double waves = std::ceil(tiles / fit);
-                double block = std::max(S * steps * mma, (S * planes * TR * rowb + planes * nt * rowb) / 56.0);
-                if (pass) block = std::max(block, planes == 3 ? 1100.0 + 6.0 * nt : 500.0 + nt);
-                const double t = waves * (3000 + std::ceil((double)p.nkb() / split) * block + out / split +
-                                          (l ? 1500 + S * rows * TR * 4 / 64.0 : rows * TR * S * 4 / 256.0));
-                if (!best.nt || t < best.cycles) best = Choice{nt, ONE, l, t};
-            }
-        }
-        if (nt <= widest && nt * 4 >= widest) {
-            const double tiles = tiles_m * ((p.tiles_n() + 1) / 2);
-            const double block = std::max(S * steps * mma * 1.15, (S * planes * TR * rowb + planes * nt / 2 * rowb) / 56.0);
-            const double work = p.nkb() * block;
-            double t = 4500 + std::ceil(tiles / (sms / 2)) * std::max(work, out) + std::min(work, out);
-            if (pass) t += 3500 + (double)M * p.K * (planes == 3 ? 10 : 4) / 3000.0;
-            if (t < best.cycles) best = Choice{nt, PAIR, 0, t};
-        }
-    }
-    return best;
-}
-
 template <class T, int PLANES, bool GATED, bool MANUAL>
 bool run_one(const Plan& pl, const Call& c, const Operands& op, const Choice& ch, cudaStream_t st) {
     if (ch.nt == 32) return launch<T, 32, PLANES, GATED, ONE, MANUAL>(pl, c, op, ch.log2_split, st);
@@ -997,14 +953,54 @@ void layout(const Plan& p, const void* w, uint8_t* tiles, float* rows, cudaStrea
     k_rows4<<<grid_for(p.N * p.k4()), 256, 0, st>>>((const float*)w, p.N, p.K, p.k4(), rows);
 }
 
-size_t tc_workspace(const Plan& p, const Call& c) {
-    if (tma_rows(p, c) || choose(p, c.M, true).mode == ONE) return 0;
+// The form and tile of a call, by an estimate of its SM cycles. Fixed parts and rates as measured
+// (clock64 stamps in the kernel): about 3000 cycles from launch to the first MMA, a K block the larger
+// of its MMAs (64 cycles each up to N = 128, N / 2 above) and its bytes at 56 a cycle, 1500 cycles for the
+// exchange in a cluster and 64 bytes a cycle stored in it, four outputs a cycle in the epilogue. Clusters of
+// 8 and 4 fit 15 and 33 times, pairs on all SMs.
+Choice choose(const Plan& p, const Call& c) {
+    const int64_t M = c.M;
+    const bool pass = !tma_rows(p, c);  // PAIR needs the rows split or packed, ONE loads them itself
+    const int S = p.gated ? 2 : 1, planes = p.planes(), rowb = planes == 3 ? 64 : 128;
+    const int steps = planes == 3 ? 12 : 4, sms = device_sm_count();
+    const int widest = planes == 3 ? 128 / S : 256 / S;  // accumulators in TMEM
+    Choice best;
+    for (int nt = 32; nt <= 256; nt *= 2) {
+        const double tiles_m = (double)((M + nt - 1) / nt), mma = std::max(64, nt / 2);
+        const double rows = std::min<double>(nt, (double)M), out = rows * TR * S / 4.0;
+        if (nt <= std::min(widest, 128)) {
+            for (int l = 0; l < 4; l++) {
+                const int split = 1 << l;
+                if (l && p.nkb() < 2 * split) break;
+                const int fit = split == 8 ? 15 : split == 4 ? 33 : sms / split;
+                const double tiles = tiles_m * p.tiles_n();
+                const double waves = std::ceil(tiles / fit);
+                double block = std::max(S * steps * mma, (S * planes * TR * rowb + planes * nt * rowb) / 56.0);
+                if (pass) block = std::max(block, planes == 3 ? 1100.0 + 6.0 * nt : 500.0 + nt);
+                const double t = waves * (3000 + std::ceil((double)p.nkb() / split) * block + out / split +
+                                          (l ? 1500 + S * rows * TR * 4 / 64.0 : rows * TR * S * 4 / 256.0));
+                if (!best.nt || t < best.cycles) best = Choice{nt, ONE, l, t};
+            }
+        }
+        if (nt <= widest && nt * 4 >= widest) {
+            const double tiles = tiles_m * ((p.tiles_n() + 1) / 2);
+            const double block = std::max(S * steps * mma * 1.15, (S * planes * TR * rowb + planes * nt / 2 * rowb) / 56.0);
+            const double work = p.nkb() * block;
+            double t = 4500 + std::ceil(tiles / (sms / 2)) * std::max(work, out) + std::min(work, out);
+            if (pass) t += 3500 + (double)M * p.K * (planes == 3 ? 10 : 4) / 3000.0;
+            if (t < best.cycles) best = Choice{nt, PAIR, 0, t};
+        }
+    }
+    return best;
+}
+
+size_t tc_workspace(const Plan& p, const Call& c, const Choice& ch) {
+    if (tma_rows(p, c) || ch.mode == ONE) return 0;
     return (size_t)p.planes() * c.M * kp_of(p) * 2;
 }
 
-int tc(const Plan& p, const Call& c, void* ws, cudaStream_t st) {
+int tc(const Plan& p, const Call& c, const Choice& ch, void* ws, cudaStream_t st) {
     const bool direct = tma_rows(p, c);
-    const Choice ch = choose(p, c.M, !direct);
     Operands op{c.x, c.ldx, p.K};
     int n = 0;
     if (!direct && ch.mode == PAIR) {

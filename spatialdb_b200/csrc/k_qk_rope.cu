@@ -45,10 +45,22 @@ struct Vec16 {
     T v[N];
 };
 
+// a / b and a % b for a below `most`, in 32 bits where they suffice (a 64-bit division costs ten times as much).
+SLX_DEV void divide(int64_t a, int b, int64_t most, int64_t& quo, int& rem) {
+    if (most < (1ll << 32)) {
+        const uint32_t q = (uint32_t)a / (uint32_t)b;
+        quo = q;
+        rem = (int)((uint32_t)a - q * (uint32_t)b);
+    } else {
+        quo = a / b;
+        rem = (int)(a - quo * b);
+    }
+}
+
 // Row m's position, or -1 when the row is to be left alone (a negative entry, or one outside the
 // table, which raises KERR_RANGE unless it is exactly -1).
 SLX_DEV int position(const QkRope& p, int64_t m) {
-    if (!p.pos) return (int)(m % p.T);
+    if (!p.pos) return p.M < (1ll << 31) && p.T < (1ll << 31) ? (int)((uint32_t)m % (uint32_t)p.T) : (int)(m % p.T);
     const int t = p.pos[m];
     if (t >= 0 && t < p.table_rows) return t;
     if (t != -1) atomicOr(p.err, KERR_RANGE);
@@ -57,21 +69,33 @@ SLX_DEV int position(const QkRope& p, int64_t m) {
 
 // 16-byte chunks. Lane j of a head's group of G lanes owns chunk j and its partner chunk j + h for
 // j < h = half / N, and past those the two unrotated chunks 2h + 2(j - h) and the next one. A group walks
-// `iters` heads of one row, so the row's table entries are read once per group.
+// `iters` heads of one row, so the row's table entries are read once per group, with the next head's
+// values in flight while this one's are worked on.
 template <class T, int G>
 __global__ void __launch_bounds__(QT) k_qk_vec(QkRope p, int slabs, int iters) {
     constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 31, j = lane & (G - 1), grp = lane / G;
     const unsigned gmask = (G == 32 ? 0xffffffffu : (1u << (G & 31)) - 1u) << (grp * G & 31);
-    const int64_t unit = (int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
-    const int64_t m = unit / slabs;
+    int64_t m;
+    int slab;
+    divide((int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5), slabs, p.M * slabs + QT, m, slab);
     if (m >= p.M) return;
-    const int head0 = (int)(unit % slabs) * iters * (32 / G) + grp;
     const int nheads = p.q.nh + p.k.nh;
     const int h = p.half / N, chunks = p.hd / N;
     const bool pair = j < h;
     const int ca = pair ? j : 2 * j, cb = pair ? j + h : 2 * j + 1;  // 2h + 2(j - h) = 2j
     const bool has_a = ca < chunks, has_b = cb < chunks;
+    int head = slab * iters * (32 / G) + grp;
+    Vec16<T> na, nb;  // the next head's values
+    auto fetch = [&](int hh) {
+        if (hh >= nheads) return;
+        const bool isq = hh < p.q.nh;
+        const T* x = isq ? (const T*)p.q.in + m * p.q.ld_in + (int64_t)hh * p.hd
+                         : (const T*)p.k.in + m * p.k.ld_in + (int64_t)(hh - p.q.nh) * p.hd;
+        if (has_a) *(uint4*)&na = *(const uint4*)(x + (int64_t)ca * N);
+        if (has_b) *(uint4*)&nb = *(const uint4*)(x + (int64_t)cb * N);
+    };
+    fetch(head);
     const int pos = position(p, m);
     if (pos < 0) return;
     float cs[N], sn[N];
@@ -82,28 +106,19 @@ __global__ void __launch_bounds__(QT) k_qk_vec(QkRope p, int slabs, int iters) {
             const float4 v = t[e / 2];
             cs[e] = v.x; sn[e] = v.y; cs[e + 1] = v.z; sn[e + 1] = v.w;
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; e++) { cs[e] = 1.0f; sn[e] = 0.0f; }
     }
     const float inv_n = 1.0f / (float)p.hd;
-    for (int i = 0; i < iters; i++) {
-        const int head = head0 + i * (32 / G);
-        const bool live = head < nheads;
-        const bool isq = head < p.q.nh;
-        const QkSide& s = isq ? p.q : p.k;
-        const int hh = isq ? head : head - p.q.nh;
-        const T* x = (const T*)s.in + m * s.ld_in + (int64_t)hh * p.hd;
-        Vec16<T> va, vb;
+    for (int i = 0; i < iters && head < nheads; i++, head += 32 / G) {
+        Vec16<T> va = na, vb = nb;
+        if (i + 1 < iters) fetch(head + 32 / G);
         float a[N], b[N];
-        if (live && has_a) *(uint4*)&va = *(const uint4*)(x + (int64_t)ca * N);
-        if (live && has_b) *(uint4*)&vb = *(const uint4*)(x + (int64_t)cb * N);
 #pragma unroll
         for (int e = 0; e < N; e++) {
-            a[e] = live && has_a ? to_f(va.v[e]) : 0.0f;
-            b[e] = live && has_b ? to_f(vb.v[e]) : 0.0f;
+            a[e] = has_a ? to_f(va.v[e]) : 0.0f;
+            b[e] = has_b ? to_f(vb.v[e]) : 0.0f;
         }
-        const float* w = (const float*)s.w;
+        const bool isq = head < p.q.nh;
+        const float* w = (const float*)(isq ? p.q.w : p.k.w);
         if (w) {  // the same for every lane of a head's group
             float ss = 0.0f;
 #pragma unroll
@@ -119,14 +134,12 @@ __global__ void __launch_bounds__(QT) k_qk_vec(QkRope p, int slabs, int iters) {
                 b[e] *= r * wb.x; b[e + 1] *= r * wb.y; b[e + 2] *= r * wb.z; b[e + 3] *= r * wb.w;
             }
         }
-        if (!live) continue;
-        T* y = (T*)s.out + m * s.ld_out + (int64_t)hh * p.hd;
+        T* y = isq ? (T*)p.q.out + m * p.q.ld_out + (int64_t)head * p.hd
+                   : (T*)p.k.out + m * p.k.ld_out + (int64_t)(head - p.q.nh) * p.hd;
 #pragma unroll
         for (int e = 0; e < N; e++) {
-            const float ya = pair ? fmaf(a[e], cs[e], -(b[e] * sn[e])) : a[e];
-            const float yb = pair ? fmaf(a[e], sn[e], b[e] * cs[e]) : b[e];
-            va.v[e] = from_f<T>(ya);
-            vb.v[e] = from_f<T>(yb);
+            va.v[e] = from_f<T>(pair ? fmaf(a[e], cs[e], -(b[e] * sn[e])) : a[e]);
+            vb.v[e] = from_f<T>(pair ? fmaf(a[e], sn[e], b[e] * cs[e]) : b[e]);
         }
         if (has_a) *(uint4*)(y + (int64_t)ca * N) = *(const uint4*)&va;
         if (has_b) *(uint4*)(y + (int64_t)cb * N) = *(const uint4*)&vb;
@@ -138,10 +151,10 @@ __global__ void __launch_bounds__(QT) k_qk_vec(QkRope p, int slabs, int iters) {
 template <class T>
 __global__ void __launch_bounds__(QT) k_qk_any(QkRope p) {
     const int lane = threadIdx.x & 31, nheads = p.q.nh + p.k.nh;
-    const int64_t unit = (int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
-    const int64_t m = unit / nheads;
+    int64_t m;
+    int head;
+    divide((int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5), nheads, p.M * nheads + QT, m, head);
     if (m >= p.M) return;
-    const int head = (int)(unit % nheads);
     const int pos = position(p, m);
     if (pos < 0) return;
     const bool isq = head < p.q.nh;
@@ -181,11 +194,12 @@ template <class T, int G>
 int launch_vec(const QkRope& p, cudaStream_t st) {
     const int per = 32 / G, nheads = p.q.nh + p.k.nh;
     const int steps = (nheads + per - 1) / per;  // group steps that cover a row's heads
-    // As many heads to a group as leave about 48 warps to every SM: at one token each group takes one
-    // head (the least latency), at many rows a row's table entries serve all of its heads.
+    // One head to a group while that leaves SMs without work (the least latency), then as many as keep
+    // about 48 warps to every SM, up to five: past that a row's table entries are hardly read again, and the
+    // last wave of longer warps costs more.
     const int64_t warps = (int64_t)device_sm_count() * 48;
-    const int iters = (int)std::max<int64_t>(1, std::min<int64_t>(steps, p.M * steps / warps));
-    const int slabs = (steps + iters - 1) / iters;
+    const int most = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(steps, 5), p.M * steps / warps));
+    const int slabs = (steps + most - 1) / most, iters = (steps + slabs - 1) / slabs;
     const int64_t units = p.M * slabs;
     k_qk_vec<T, G><<<(unsigned)((units + QT / 32 - 1) / (QT / 32)), QT, 0, st>>>(p, slabs, iters);
     return 1;
@@ -212,15 +226,40 @@ int launch_float(const QkRope& p, cudaStream_t st) {
 
 // ---- Q30 -------------------------------------------------------------------------------------------
 
-// RmsNormRow's root for a head's wrapping sum of squares; skip: the row is left as it is (ms <= 0).
+// RmsNormRow's root for a head's wrapping sum of squares; skip: the row is left as it is (ms <= 0). A mean
+// square below 2^62 (values below 2 in Q30) takes 64-bit arithmetic: its quotient from a double estimate (off by
+// at most 2^10), corrected by the exact remainder, and its root from a double one, corrected by squaring.
 SLX_DEV int64_t q30_root(u128 ss, int n, bool& skip) {
     skip = (i128)ss < (i128)n;
     if (skip) return 1;
+    if ((ss >> 62) < (u128)(uint32_t)n) {
+        const double rn = 1.0 / (double)n;
+        const double sd = (double)(uint64_t)(ss >> 64) * 18446744073709551616.0 + (double)(uint64_t)ss;
+        uint64_t ms = (uint64_t)(sd * rn);
+        const int64_t rem = (int64_t)((uint64_t)ss - ms * (uint64_t)n);  // exact: the true value is small
+        ms += (uint64_t)(int64_t)floor((double)rem * rn);
+        int64_t left = (int64_t)((uint64_t)ss - ms * (uint64_t)n);
+        while (left < 0) { ms--; left += n; }
+        while (left >= n) { ms++; left -= n; }
+        uint64_t r = (uint64_t)sqrt((double)ms);
+        while (r * r > ms) r--;
+        while ((r + 1) * (r + 1) <= ms) r++;
+        return r == 0 ? 1 : (int64_t)r;
+    }
     const int64_t r = isqrt_u128(udiv128_u32(ss, (uint32_t)n, ~0ULL / (uint32_t)n));
     return r == 0 ? 1 : r;
 }
 
+// floor((a c - b s) / 2^30) and floor((a s + b c) / 2^30). With c, s a Q30 cosine and sine (c^2 + s^2 <= 2^60) and
+// |a|, |b| < 6e9 the sums stay below sqrt(a^2 + b^2) 2^30 < 2^63: wrapping 64-bit arithmetic is exact.
 SLX_DEV void q30_rotate(int64_t a, int64_t b, int64_t c, int64_t s, int64_t& ya, int64_t& yb) {
+    constexpr int64_t lim = 6000000000ll;
+    if (a > -lim && a < lim && b > -lim && b < lim) {
+        const int64_t c32 = (int32_t)c, s32 = (int32_t)s;
+        ya = wsub(wmul(a, c32), wmul(b, s32)) >> 30;
+        yb = wadd(wmul(a, s32), wmul(b, c32)) >> 30;
+        return;
+    }
     ya = lo64(sar128((i128)((u128)((i128)a * c) - (u128)((i128)b * s)), 30));
     yb = lo64(sar128((i128)((u128)((i128)a * s) + (u128)((i128)b * c)), 30));
 }
@@ -229,10 +268,10 @@ SLX_DEV void q30_rotate(int64_t a, int64_t b, int64_t c, int64_t s, int64_t& ya,
 template <int PL>
 __global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
     const int lane = threadIdx.x & 31, nheads = p.q.nh + p.k.nh;
-    const int64_t unit = (int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
-    const int64_t m = unit / nheads;
+    int64_t m;
+    int head;
+    divide((int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5), nheads, p.M * nheads + QT, m, head);
     if (m >= p.M) return;
-    const int head = (int)(unit % nheads);
     const int pos = position(p, m);
     if (pos < 0) return;
     const bool isq = head < p.q.nh;
@@ -254,8 +293,19 @@ __global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
     double rd = 1.0;
     if (w) {
         u128 ss = 0;
+        bool narrow = true;  // every |x| below 2^32: a square is one 32-bit product
 #pragma unroll
-        for (int e = 0; e < PL; e++) ss += (u128)((i128)a[e] * a[e]) + (u128)((i128)b[e] * b[e]);
+        for (int e = 0; e < PL; e++) {
+            const uint64_t ua = a[e] < 0 ? 0 - (uint64_t)a[e] : (uint64_t)a[e], ub = b[e] < 0 ? 0 - (uint64_t)b[e] : (uint64_t)b[e];
+            narrow = narrow && ((ua | ub) >> 32) == 0;
+            ss += (u128)((uint64_t)(uint32_t)ua * (uint32_t)ua);
+            ss += (u128)((uint64_t)(uint32_t)ub * (uint32_t)ub);
+        }
+        if (!narrow) {
+            ss = 0;
+#pragma unroll
+            for (int e = 0; e < PL; e++) ss += (u128)((i128)a[e] * a[e]) + (u128)((i128)b[e] * b[e]);
+        }
         root = q30_root(warp_sum_u128(ss), p.hd, skip);
         rd = 1.0 / (double)root;
     }
@@ -276,10 +326,10 @@ __global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
 // Heads wider than the registers of k_qk_q30 hold: the row is read again after its norm is known.
 __global__ void __launch_bounds__(QT) k_qk_q30_wide(QkRope p) {
     const int lane = threadIdx.x & 31, nheads = p.q.nh + p.k.nh;
-    const int64_t unit = (int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
-    const int64_t m = unit / nheads;
+    int64_t m;
+    int head;
+    divide((int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5), nheads, p.M * nheads + QT, m, head);
     if (m >= p.M) return;
-    const int head = (int)(unit % nheads);
     const int pos = position(p, m);
     if (pos < 0) return;
     const bool isq = head < p.q.nh;

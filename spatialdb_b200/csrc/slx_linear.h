@@ -58,10 +58,16 @@ void layout(const Plan& p, const void* w, uint8_t* tiles, float* rows, cudaStrea
 bool few_supported(const Plan& p, int64_t M);
 int few(const Plan& p, const Call& c, cudaStream_t st);
 
-// The tensor-core product (k_linear_tc.cu). ws: tc_workspace() bytes (0: none), laid out by the call.
-// Returns the kernels queued, -1 when a tensor map could not be encoded or a launch failed.
-size_t tc_workspace(const Plan& p, const Call& c);
-int tc(const Plan& p, const Call& c, void* ws, cudaStream_t st);
+// The tensor-core product (k_linear_tc.cu): its form and tile for a call, the scratch that form needs (0: none),
+// laid out by the call, and the call itself, which returns the kernels queued, -1 when a tensor map could not
+// be encoded or a launch failed.
+struct Choice {
+    int nt = 0, mode = 0, log2_split = 0;
+    double cycles = 0;
+};
+Choice choose(const Plan& p, const Call& c);
+size_t tc_workspace(const Plan& p, const Call& c, const Choice& ch);
+int tc(const Plan& p, const Call& c, const Choice& ch, void* ws, cudaStream_t st);
 
 }  // namespace lin
 }  // namespace slx

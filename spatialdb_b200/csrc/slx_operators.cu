@@ -207,43 +207,44 @@ slx_status slx_linear_info(slx_linear* l, int64_t* info, int n) {
     return SLX_OK;
 }
 
-slx_status slx_linear_device(slx_linear* l, const void* d_x, int64_t ldx, int64_t M, const void* d_residual, int64_t ldr,
-                             void* d_y, int64_t ldy, void* stream) {
+slx_status slx_linear_device(slx_linear* l, const slx_linear_args* a) {
     if (!l) return SLX_EINVAL;
     slx_ctx* ctx = l->ctx;
+    if (!a) return set_err(ctx, SLX_EINVAL, "null argument");
     const lin::Plan& p = l->plan;
+    const int64_t M = a->M;
     if (M < 0) return set_err(ctx, SLX_EINVAL, "M %lld < 0", (long long)M);
     if (M == 0) return SLX_OK;
     const int e = width_of(p.dtype);
-    if (!d_x || !d_y) return set_err(ctx, SLX_EINVAL, "null argument");
-    if (ldx < p.K || ldy < p.N || (d_residual && ldr < p.N))
+    if (!a->x || !a->y) return set_err(ctx, SLX_EINVAL, "null argument");
+    if (a->ldx < p.K || a->ldy < p.N || (a->residual && a->ldr < p.N))
         return set_err(ctx, SLX_EINVAL, "row stride below the row's width (K %d, N %d)", p.K, p.N);
-    if (((uintptr_t)d_x | (uintptr_t)d_y | (uintptr_t)d_residual) % e)
+    if (((uintptr_t)a->x | (uintptr_t)a->y | (uintptr_t)a->residual) % e)
         return set_err(ctx, SLX_EINVAL, "rows not aligned to %d bytes", e);
-    if (M > (1 << 30) || (M + 31) / 32 * p.tiles_n() > (1ll << 30))
-        return set_err(ctx, SLX_EINVAL, "M %lld with N %d", (long long)M, p.N);
+    if (M > (1 << 30) || (M + 31) / 32 * p.tiles_n() > (1ll << 27) || a->ldx > (1ll << 36))
+        return set_err(ctx, SLX_EINVAL, "M %lld with N %d, row stride %lld", (long long)M, p.N, (long long)a->ldx);
     OnDevice on(ctx->device);
     CK(on.err);
-    cudaStream_t st = pick(ctx, stream);
+    cudaStream_t st = pick(ctx, a->stream);
     lin::Call c;
-    c.x = d_x; c.ldx = ldx; c.r = d_residual; c.ldr = ldr; c.y = d_y; c.ldo = ldy; c.M = M;
+    c.x = a->x; c.ldx = a->ldx; c.r = a->residual; c.ldr = a->ldr; c.y = a->y; c.ldo = a->ldy; c.M = M;
     c.err = ctx->d_flag;
     c.wait_limit = ctx->wait.limit_cycles;
     c.stall_mma = ctx->wait.stall_mma;
     const double macs = (double)M * p.N * p.K * (p.gated ? 2 : 1);
-    const double bytes = (double)e * (M * p.K + (double)p.N * p.K * (p.gated ? 2 : 1) + M * p.N * (d_residual ? 2 : 1));
+    const double bytes = (double)e * (M * p.K + (double)p.N * p.K * (p.gated ? 2 : 1) + M * p.N * (a->residual ? 2 : 1));
     if (lin::few_supported(p, M)) {
         run_k(ctx, KC_GEMV, macs, bytes, st, [&] { return lin::few(p, c, st); });
         CK(cudaGetLastError());
         return SLX_OK;
     }
-    const size_t need = lin::tc_workspace(p, c);
+    const lin::Choice ch = lin::choose(p, c);
     void* ws = nullptr;
-    if (need) {
+    if (const size_t need = lin::tc_workspace(p, c, ch)) {
         if (int rc = scratch(ctx, need, st, &ws)) return rc;
     }
     int n = 0;
-    run_k(ctx, KC_GEMM, macs, bytes, st, [&] { return (n = lin::tc(p, c, ws, st)) < 0 ? 0 : n; });
+    run_k(ctx, KC_GEMM, macs, bytes, st, [&] { return (n = lin::tc(p, c, ch, ws, st)) < 0 ? 0 : n; });
     const cudaError_t launched = cudaGetLastError();
     if (ws) CK(cudaFreeAsync(ws, st));
     if (launched != cudaSuccess || n < 0)
@@ -341,33 +342,34 @@ slx_status slx_qk_norm_free(slx_qk_norm* h) {
     return SLX_OK;
 }
 
-slx_status slx_qk_norm_rope_device(slx_qk_norm* h, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, int64_t M,
-                                   int64_t T, const int32_t* d_pos, void* d_qo, int64_t ldqo, void* d_ko, int64_t ldko,
-                                   void* stream) {
+slx_status slx_qk_norm_rope_device(slx_qk_norm* h, const slx_qk_args* a) {
     if (!h) return SLX_EINVAL;
     slx_ctx* ctx = h->ctx;
+    if (!a) return set_err(ctx, SLX_EINVAL, "null argument");
     const slx_rope* r = h->rope;
+    const int64_t M = a->M, T = a->T;
     if (M < 0) return set_err(ctx, SLX_EINVAL, "M %lld < 0", (long long)M);
     if (M == 0) return SLX_OK;
     const int e = width_of(h->dtype);
     const int64_t nq = (int64_t)h->heads * h->hd, nk = (int64_t)h->kv_heads * h->hd;
-    if ((nq && (!d_q || !d_qo)) || (nk && (!d_k || !d_ko))) return set_err(ctx, SLX_EINVAL, "null argument");
-    if ((nq && (ldq < nq || ldqo < nq)) || (nk && (ldk < nk || ldko < nk)))
+    if ((nq && (!a->q || !a->qo)) || (nk && (!a->k || !a->ko))) return set_err(ctx, SLX_EINVAL, "null argument");
+    if ((nq && (a->ldq < nq || a->ldqo < nq)) || (nk && (a->ldk < nk || a->ldko < nk)))
         return set_err(ctx, SLX_EINVAL, "row stride below the row's width (q %lld, k %lld)", (long long)nq, (long long)nk);
-    if (((nq ? (uintptr_t)d_q | (uintptr_t)d_qo : 0) | (nk ? (uintptr_t)d_k | (uintptr_t)d_ko : 0)) % e)
+    if (((nq ? (uintptr_t)a->q | (uintptr_t)a->qo : 0) | (nk ? (uintptr_t)a->k | (uintptr_t)a->ko : 0)) % e)
         return set_err(ctx, SLX_EINVAL, "rows not aligned to %d bytes", e);
-    if ((uintptr_t)d_pos % 4) return set_err(ctx, SLX_EINVAL, "positions not aligned to 4 bytes");
-    if (!d_pos && T <= 0) return set_err(ctx, SLX_EINVAL, "sequence length %lld", (long long)T);
-    if (!d_pos && std::min(T, M) > r->rows)
+    if ((uintptr_t)a->pos % 4) return set_err(ctx, SLX_EINVAL, "positions not aligned to 4 bytes");
+    if (!a->pos && T <= 0) return set_err(ctx, SLX_EINVAL, "sequence length %lld", (long long)T);
+    if (!a->pos && std::min(T, M) > r->rows)
         return set_err(ctx, SLX_ERANGE, "sequence length %lld exceeds the RoPE table (%d rows)", (long long)T, r->rows);
-    if (M > (1ll << 33) / (h->heads + h->kv_heads)) return set_err(ctx, SLX_EINVAL, "M %lld rows of %d heads", (long long)M, h->heads + h->kv_heads);
+    if (M > (1ll << 33) / (h->heads + h->kv_heads))
+        return set_err(ctx, SLX_EINVAL, "M %lld rows of %d heads", (long long)M, h->heads + h->kv_heads);
     OnDevice on(ctx->device);
     CK(on.err);
-    cudaStream_t st = pick(ctx, stream);
+    cudaStream_t st = pick(ctx, a->stream);
     QkRope p;
-    p.q.in = d_q; p.q.out = d_qo; p.q.ld_in = ldq; p.q.ld_out = ldqo; p.q.nh = h->heads; p.q.w = h->wq;
-    p.k.in = d_k; p.k.out = d_ko; p.k.ld_in = ldk; p.k.ld_out = ldko; p.k.nh = h->kv_heads; p.k.w = h->wk;
-    p.hd = h->hd; p.half = r->rot / 2; p.M = M; p.T = T; p.pos = d_pos;
+    p.q.in = a->q; p.q.out = a->qo; p.q.ld_in = a->ldq; p.q.ld_out = a->ldqo; p.q.nh = h->heads; p.q.w = h->wq;
+    p.k.in = a->k; p.k.out = a->ko; p.k.ld_in = a->ldk; p.k.ld_out = a->ldko; p.k.nh = h->kv_heads; p.k.w = h->wk;
+    p.hd = h->hd; p.half = r->rot / 2; p.M = M; p.T = T; p.pos = a->pos;
     p.table_rows = r->rows; p.table = r->table; p.cs = r->cs; p.sn = r->sn;
     p.eps = h->eps; p.err = ctx->d_flag;
     run_k(ctx, KC_ROPE, 0, 2.0 * e * M * (nq + nk), st,

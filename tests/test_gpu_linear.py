@@ -353,7 +353,7 @@ def test_handle_outlives_its_context():
     lib.slx_destroy(own._h)
     own._h = None
     c.op._h = None
-    assert lib.slx_linear_device(h, c.x.data_ptr(), 64, 20, None, 64, c.y.data_ptr(), 64, slx.STREAM_LEGACY) == 0
+    assert lib.slx_linear_device(h, slx._LINEAR_ARGS(c.x.data_ptr(), 64, 20, 0, 64, c.y.data_ptr(), 64, slx.STREAM_LEGACY)) == 0
     torch.cuda.synchronize()
     y, e = c.want()
     assert bool(((c.y.double() - y).abs() <= e).all())

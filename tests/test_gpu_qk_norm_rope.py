@@ -266,8 +266,8 @@ def test_table_and_context_freed_first():
     lib, h = own._lib, c.op._h
     lib.slx_destroy(own._h)
     own._h = c.op._h = None
-    a = (c.q.data_ptr(), 128, c.k.data_ptr(), 64, 5, 5, None, c.qo.data_ptr(), 128, c.ko.data_ptr(), 64, slx.STREAM_LEGACY)
-    assert lib.slx_qk_norm_rope_device(h, *a) == 0
+    a = (c.q.data_ptr(), 128, c.k.data_ptr(), 64, 5, 5, 0, c.qo.data_ptr(), 128, c.ko.data_ptr(), 64, slx.STREAM_LEGACY)
+    assert lib.slx_qk_norm_rope_device(h, slx._QK_ARGS(*a)) == 0
     torch.cuda.synchronize()
     (y, e), _ = c.want()
     assert bool(((c.qo.double() - y).abs() <= e).all())
