@@ -26,6 +26,7 @@ namespace slx {
 namespace {
 
 constexpr int QT = 256;  // threads per block
+constexpr int QV = 128;  // of k_qk_vec
 
 SLX_DEV float to_f(float v) { return v; }
 SLX_DEV float to_f(__half v) { return __half2float(v); }
@@ -39,11 +40,69 @@ SLX_DEV __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <>
 SLX_DEV __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two fp32 values in a 64-bit register: the packed FMA and multiply do both in one instruction.
+typedef unsigned long long f32x2;
+SLX_DEV f32x2 pack2(float lo, float hi) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+SLX_DEV void unpack2(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+SLX_DEV f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+SLX_DEV f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
+// 16 bytes of a row as pairs of fp32 values, and back with one rounding.
 template <class T>
 struct Vec16 {
     static constexpr int N = 16 / sizeof(T);
-    T v[N];
+    uint4 raw;
 };
+SLX_DEV void widen(const Vec16<float>& v, f32x2 (&o)[2]) {
+    o[0] = pack2(__uint_as_float(v.raw.x), __uint_as_float(v.raw.y));
+    o[1] = pack2(__uint_as_float(v.raw.z), __uint_as_float(v.raw.w));
+}
+SLX_DEV f32x2 widen2(uint32_t w, __nv_bfloat16) { return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+SLX_DEV f32x2 widen2(uint32_t w, __half) {
+    const float2 f = __half22float2(*(const __half2*)&w);
+    return pack2(f.x, f.y);
+}
+template <class T>
+SLX_DEV void widen(const Vec16<T>& v, f32x2 (&o)[4]) {
+    o[0] = widen2(v.raw.x, T());
+    o[1] = widen2(v.raw.y, T());
+    o[2] = widen2(v.raw.z, T());
+    o[3] = widen2(v.raw.w, T());
+}
+SLX_DEV uint32_t narrow2(f32x2 v, __nv_bfloat16) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *(const uint32_t*)&h;
+}
+SLX_DEV uint32_t narrow2(f32x2 v, __half) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *(const uint32_t*)&h;
+}
+SLX_DEV uint4 narrow(const f32x2 (&v)[2], float) {
+    float f[4];
+    unpack2(v[0], f[0], f[1]);
+    unpack2(v[1], f[2], f[3]);
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+template <class T>
+SLX_DEV uint4 narrow(const f32x2 (&v)[4], T t) {
+    return make_uint4(narrow2(v[0], t), narrow2(v[1], t), narrow2(v[2], t), narrow2(v[3], t));
+}
 
 // a / b and a % b for a below `most`, in 32 bits where they suffice (a 64-bit division costs ten times as much).
 SLX_DEV void divide(int64_t a, int b, int64_t most, int64_t& quo, int& rem) {
@@ -68,81 +127,98 @@ SLX_DEV int position(const QkRope& p, int64_t m) {
 }
 
 // 16-byte chunks. Lane j of a head's group of G lanes owns chunk j and its partner chunk j + h for
-// j < h = half / N, and past those the two unrotated chunks 2h + 2(j - h) and the next one. A group walks
-// `iters` heads of one row, so the row's table entries are read once per group, with the next head's
-// values in flight while this one's are worked on.
-template <class T, int G>
-__global__ void __launch_bounds__(QT) k_qk_vec(QkRope p, int slabs, int iters) {
+// j < h = half / N, and past those the two unrotated chunks 2h + 2(j - h) and the next one. A warp takes one
+// row's query heads or key heads, 32 / G at a time in up to STEPS steps: the row's table entries are read once.
+// Every step's values are asked for before the position is known, so that a warp has up to STEPS KB in flight
+// while it waits for the position and then for the table (with one step in flight at a time 24 warps an SM
+// kept 24 KB in flight, where the memory's rate times its latency is about 44).
+struct Slabs {
+    int q, k;  // warps to a row's query and key heads
+};
+template <class T, int G, int STEPS>
+__global__ void __launch_bounds__(QV) k_qk_vec(QkRope p, Slabs sl) {
     constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 31, j = lane & (G - 1), grp = lane / G;
     const unsigned gmask = (G == 32 ? 0xffffffffu : (1u << (G & 31)) - 1u) << (grp * G & 31);
     int64_t m;
     int slab;
-    divide((int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5), slabs, p.M * slabs + QT, m, slab);
+    divide((int64_t)blockIdx.x * (QV / 32) + (threadIdx.x >> 5), sl.q + sl.k, p.M * (sl.q + sl.k) + QV, m, slab);
     if (m >= p.M) return;
-    const int nheads = p.q.nh + p.k.nh;
+    const bool isq = slab < sl.q;
+    const QkSide& s = isq ? p.q : p.k;
+    constexpr int PER = 32 / G;
+    const int head = (isq ? slab : slab - sl.q) * STEPS * PER + grp;
     const int h = p.half / N, chunks = p.hd / N;
     const bool pair = j < h;
     const int ca = pair ? j : 2 * j, cb = pair ? j + h : 2 * j + 1;  // 2h + 2(j - h) = 2j
     const bool has_a = ca < chunks, has_b = cb < chunks;
-    int head = slab * iters * (32 / G) + grp;
-    Vec16<T> na, nb;  // the next head's values
-    auto fetch = [&](int hh) {
-        if (hh >= nheads) return;
-        const bool isq = hh < p.q.nh;
-        const T* x = isq ? (const T*)p.q.in + m * p.q.ld_in + (int64_t)hh * p.hd
-                         : (const T*)p.k.in + m * p.k.ld_in + (int64_t)(hh - p.q.nh) * p.hd;
-        if (has_a) *(uint4*)&na = *(const uint4*)(x + (int64_t)ca * N);
-        if (has_b) *(uint4*)&nb = *(const uint4*)(x + (int64_t)cb * N);
-    };
-    fetch(head);
+    const T* x = (const T*)s.in + m * s.ld_in + (int64_t)head * p.hd;
+    T* y = (T*)s.out + m * s.ld_out + (int64_t)head * p.hd;
+    Vec16<T> va[STEPS], vb[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        const bool live = head + i * PER < s.nh;
+        const T* from = x + (int64_t)i * PER * p.hd;
+        va[i].raw = live && has_a ? *(const uint4*)(from + ca * N) : make_uint4(0, 0, 0, 0);
+        vb[i].raw = live && has_b ? *(const uint4*)(from + cb * N) : make_uint4(0, 0, 0, 0);
+    }
     const int pos = position(p, m);
     if (pos < 0) return;
-    float cs[N], sn[N];
+    constexpr int P = N / 2;
+    f32x2 cs[P], sn[P], ns[P];  // cosines, sines and the sines' negatives
     if (pair) {
         const float4* t = (const float4*)(p.table + (int64_t)pos * p.half + (int64_t)j * N);
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-            const float4 v = t[e / 2];
-            cs[e] = v.x; sn[e] = v.y; cs[e + 1] = v.z; sn[e + 1] = v.w;
+        for (int e = 0; e < P; e++) {
+            const float4 v = t[e];
+            cs[e] = pack2(v.x, v.z);
+            sn[e] = pack2(v.y, v.w);
+            ns[e] = pack2(-v.y, -v.w);
         }
     }
     const float inv_n = 1.0f / (float)p.hd;
-    for (int i = 0; i < iters && head < nheads; i++, head += 32 / G) {
-        Vec16<T> va = na, vb = nb;
-        if (i + 1 < iters) fetch(head + 32 / G);
-        float a[N], b[N];
+    const float* w = (const float*)s.w;
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            a[e] = has_a ? to_f(va.v[e]) : 0.0f;
-            b[e] = has_b ? to_f(vb.v[e]) : 0.0f;
-        }
-        const bool isq = head < p.q.nh;
-        const float* w = (const float*)(isq ? p.q.w : p.k.w);
-        if (w) {  // the same for every lane of a head's group
-            float ss = 0.0f;
+    for (int i = 0; i < STEPS; i++, y += PER * p.hd) {
+        if (head + i * PER >= s.nh) break;
+        f32x2 a[P], b[P];
+        widen(va[i], a);
+        widen(vb[i], b);
+        if (w) {
+            f32x2 sq = 0;  // 0.0, 0.0
 #pragma unroll
-            for (int e = 0; e < N; e++) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
+            for (int e = 0; e < P; e++) sq = fma2(a[e], a[e], fma2(b[e], b[e], sq));
+            float lo, hi;
+            unpack2(sq, lo, hi);
+            float ss = lo + hi;
 #pragma unroll
             for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(gmask, ss, o);
-            const float r = 1.0f / sqrtf(fmaf(ss, inv_n, p.eps));
+            const float r1 = rsqrtf(fmaf(ss, inv_n, p.eps));
+            const f32x2 r = pack2(r1, r1);
 #pragma unroll
-            for (int e = 0; e < N; e += 4) {
-                const float4 wa = has_a ? *(const float4*)(w + ca * N + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const float4 wb = has_b ? *(const float4*)(w + cb * N + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                a[e] *= r * wa.x; a[e + 1] *= r * wa.y; a[e + 2] *= r * wa.z; a[e + 3] *= r * wa.w;
-                b[e] *= r * wb.x; b[e + 1] *= r * wb.y; b[e + 2] *= r * wb.z; b[e + 3] *= r * wb.w;
+            for (int e = 0; e < P; e += 2) {
+                if (has_a) {
+                    const float4 v = *(const float4*)(w + ca * N + 2 * e);
+                    a[e] = mul2(a[e], mul2(r, pack2(v.x, v.y)));
+                    a[e + 1] = mul2(a[e + 1], mul2(r, pack2(v.z, v.w)));
+                }
+                if (has_b) {
+                    const float4 v = *(const float4*)(w + cb * N + 2 * e);
+                    b[e] = mul2(b[e], mul2(r, pack2(v.x, v.y)));
+                    b[e + 1] = mul2(b[e + 1], mul2(r, pack2(v.z, v.w)));
+                }
             }
         }
-        T* y = isq ? (T*)p.q.out + m * p.q.ld_out + (int64_t)head * p.hd
-                   : (T*)p.k.out + m * p.k.ld_out + (int64_t)(head - p.q.nh) * p.hd;
+        if (pair) {
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            va.v[e] = from_f<T>(pair ? fmaf(a[e], cs[e], -(b[e] * sn[e])) : a[e]);
-            vb.v[e] = from_f<T>(pair ? fmaf(a[e], sn[e], b[e] * cs[e]) : b[e]);
+            for (int e = 0; e < P; e++) {
+                const f32x2 t = fma2(a[e], cs[e], mul2(b[e], ns[e]));
+                b[e] = fma2(a[e], sn[e], mul2(b[e], cs[e]));
+                a[e] = t;
+            }
         }
-        if (has_a) *(uint4*)(y + (int64_t)ca * N) = *(const uint4*)&va;
-        if (has_b) *(uint4*)(y + (int64_t)cb * N) = *(const uint4*)&vb;
+        if (has_a) *(uint4*)(y + ca * N) = narrow(a, T());
+        if (has_b) *(uint4*)(y + cb * N) = narrow(b, T());
     }
 }
 
@@ -171,7 +247,7 @@ __global__ void __launch_bounds__(QT) k_qk_any(QkRope p) {
             ss = fmaf(v, v, ss);
         }
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        r = 1.0f / sqrtf(fmaf(ss, 1.0f / (float)p.hd, p.eps));
+        r = rsqrtf(fmaf(ss, 1.0f / (float)p.hd, p.eps));
     }
     const float2* t = p.table + (int64_t)pos * p.half;
     for (int i = lane; i < p.half; i += 32) {
@@ -190,19 +266,23 @@ __global__ void __launch_bounds__(QT) k_qk_any(QkRope p) {
     }
 }
 
+template <class T, int G, int STEPS>
+int launch_steps(const QkRope& p, cudaStream_t st) {
+    const int heads = 32 / G * STEPS;  // of a warp
+    const Slabs sl{(p.q.nh + heads - 1) / heads, (p.k.nh + heads - 1) / heads};
+    const int64_t units = p.M * (sl.q + sl.k);
+    k_qk_vec<T, G, STEPS><<<(unsigned)((units + QV / 32 - 1) / (QV / 32)), QV, 0, st>>>(p, sl);
+    return 1;
+}
+// One step to a warp while that leaves SMs without work (the least latency), then two and four (f16 3001 x (20 + 4) x
+// 96, in us with 1, 2, 3, 4 steps: 12.3, 10.3, 12.3, 14.4; bf16 8192 x (32 + 8) x 128: 44.6, 36.9, 39.7, 36.9).
 template <class T, int G>
 int launch_vec(const QkRope& p, cudaStream_t st) {
-    const int per = 32 / G, nheads = p.q.nh + p.k.nh;
-    const int steps = (nheads + per - 1) / per;  // group steps that cover a row's heads
-    // One head to a group while that leaves SMs without work (the least latency), then as many as keep
-    // about 48 warps to every SM, up to five: past that a row's table entries are hardly read again, and the
-    // last wave of longer warps costs more.
-    const int64_t warps = (int64_t)device_sm_count() * 48;
-    const int most = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(steps, 5), p.M * steps / warps));
-    const int slabs = (steps + most - 1) / most, iters = (steps + slabs - 1) / slabs;
-    const int64_t units = p.M * slabs;
-    k_qk_vec<T, G><<<(unsigned)((units + QT / 32 - 1) / (QT / 32)), QT, 0, st>>>(p, slabs, iters);
-    return 1;
+    const int per = 32 / G;
+    const int64_t steps = p.M * ((p.q.nh + per - 1) / per + (p.k.nh + per - 1) / per), warps = (int64_t)device_sm_count() * 20;
+    if (steps < 2 * warps) return launch_steps<T, G, 1>(p, st);
+    if (steps < 12 * warps) return launch_steps<T, G, 2>(p, st);
+    return launch_steps<T, G, 4>(p, st);
 }
 
 template <class T>
@@ -264,6 +344,26 @@ SLX_DEV void q30_rotate(int64_t a, int64_t b, int64_t c, int64_t s, int64_t& ya,
     yb = lo64(sar128((i128)((u128)((i128)a * s) + (u128)((i128)b * c)), 30));
 }
 
+// trunc(x w / root) for a value of a row whose |x| are all below 2^32 and whose root is `root`: muldiv_trunc with
+// one range check. sum x^2 < n (root + 1)^2, so |x| < 2 sqrt(n) root and the quotient is below 2 sqrt(n) |w|: for
+// |w| < 2^43 and n <= 512 below 2^49, muldiv_trunc's own bound for its estimate.
+SLX_DEV int64_t q30_scale(int64_t x, int64_t w, int64_t root, double rd) {
+    const bool minus = (x ^ w) < 0;
+    const uint64_t uw = w < 0 ? 0 - (uint64_t)w : (uint64_t)w;
+    const uint32_t ux = (uint32_t)(x < 0 ? -x : x);
+    if (uw >= (1ull << 43)) return muldiv_trunc(x, w, d_i64(w), root, rd);
+    const double P = d_u32(ux) * d_i64((int64_t)uw);
+    const double y = rd_floor(P, rd);
+    int64_t q = rd_i64(y);
+    const double fl = y - RD_BASE, frac = __fma_rn(P, rd, -fl), tol = __fma_rn(fl, 0x1p-50, 0x1p-50);
+    if (frac < tol || frac > 1.0 - tol) {
+        int64_t r = (int64_t)(ux * uw - (uint64_t)q * (uint64_t)root);
+        while (r < 0) { q--; r += root; }
+        while (r >= root) { q++; r -= root; }
+    }
+    return minus ? -q : q;
+}
+
 // One warp per head row, lane l owning the pairs l, l + 32, ... (PL of them, held in registers).
 template <int PL>
 __global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
@@ -288,12 +388,11 @@ __global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
         a[e] = i < p.half ? x[i] : 0;
         b[e] = i < p.half ? x[i + p.half] : 0;
     }
-    bool skip = true;
+    bool skip = true, narrow = true;  // narrow: every |x| of the lane below 2^32, a square is one 32-bit product
     int64_t root = 1;
     double rd = 1.0;
     if (w) {
         u128 ss = 0;
-        bool narrow = true;  // every |x| below 2^32: a square is one 32-bit product
 #pragma unroll
         for (int e = 0; e < PL; e++) {
             const uint64_t ua = a[e] < 0 ? 0 - (uint64_t)a[e] : (uint64_t)a[e], ub = b[e] < 0 ? 0 - (uint64_t)b[e] : (uint64_t)b[e];
@@ -316,8 +415,13 @@ __global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
         int64_t u = a[e], v = b[e];
         if (!skip) {
             const int64_t wu = w[i], wv = w[i + p.half];
-            u = muldiv_trunc(u, wu, d_i64(wu), root, rd);
-            v = muldiv_trunc(v, wv, d_i64(wv), root, rd);
+            if (narrow) {
+                u = q30_scale(u, wu, root, rd);
+                v = q30_scale(v, wv, root, rd);
+            } else {
+                u = muldiv_trunc(u, wu, d_i64(wu), root, rd);
+                v = muldiv_trunc(v, wv, d_i64(wv), root, rd);
+            }
         }
         q30_rotate(u, v, cs[i], sn[i], y[i], y[i + p.half]);
     }
