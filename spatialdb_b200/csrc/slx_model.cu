@@ -465,8 +465,8 @@ int prepare_gemms(slx_ctx* ctx, slx_model* m) {
 }
 
 // Attention for one layer: tensor-core scores when the shape allows (exact kernel gated behind).
-// q and k are rotated in place first (ApplyRoPE with the cos / sin tables): by the tensor-core path's
-// digit split itself, or by k_rope before the exact kernel.
+// With cos / sin tables q and k are rotated in place first (ApplyRoPE): by the tensor-core path's digit
+// split itself, or by k_rope before the exact kernel. Without, they come rotated.
 // With planes ([5][mpad][kpad], kpad == nh * hd) the tensor-core path also writes the output rows'
 // activation digit planes for the next projection and sets *planes_flag to the word that must stay
 // zero for them to be used; otherwise *planes_flag is left null.
@@ -488,8 +488,11 @@ int attend(slx_model* m, int64_t* q, int64_t ldq, int64_t* k, int64_t ldk, const
             }
         }
     }
-    int n = rope_rows(q, ldq, B, T, nh, hd, cs, sn, st);
-    n += rope_rows(k, ldk, B, T, nkv, hd, cs, sn, st);
+    int n = 0;
+    if (cs) {
+        n += rope_rows(q, ldq, B, T, nh, hd, cs, sn, st);
+        n += rope_rows(k, ldk, B, T, nkv, hd, cs, sn, st);
+    }
     return n + attention(q, ldq, k, ldk, v, ldv, out, ldo, B, T, nh, nkv, hd, sshift, sq, mode, window, st);
 }
 
@@ -703,15 +706,20 @@ int causal_hidden(slx_model* m, const int32_t* ids, int B, int T, int n_layers, 
             const int64_t ld3[3] = {qd, kvd, kvd};
             project_multi(m, xn, d, M, 3, ws3, ps3, cs3, ld3, st);
         }
-        RUN(KC_NORM, 0, 0, rmsnorm_rows(q, qd, M * m->heads, m->heads, hd, l.qn, st));
-        RUN(KC_NORM, 0, 0, rmsnorm_rows(k, kvd, M * m->kv_heads, m->kv_heads, hd, l.kn, st));
-        const int64_t* cs = global ? m->cos_g : m->cos_l;
-        const int64_t* sn = global ? m->sin_g : m->sin_l;
+        // RmsNormPerHead of q and k and ApplyRoPE, one launch in place
+        QkRope qk;
+        qk.q.in = qk.q.out = q; qk.q.ld_in = qk.q.ld_out = qd; qk.q.nh = m->heads; qk.q.w = l.qn;
+        qk.k.in = qk.k.out = k; qk.k.ld_in = qk.k.ld_out = kvd; qk.k.nh = m->kv_heads; qk.k.w = l.kn;
+        qk.hd = hd; qk.half = hd / 2; qk.M = M; qk.T = T;
+        qk.table_rows = m->rope_rows;
+        qk.cs = global ? m->cos_g : m->cos_l;
+        qk.sn = global ? m->sin_g : m->sin_l;
+        RUN(KC_ROPE, 0, 0, qk_norm_rope_q30(qk, st));
         int mode = !causal ? 0 : ((global || m->sliding <= 0) ? 1 : 2);
         const int* aflag = nullptr;
         RUN(KC_ATTENTION, 2.0 * B * m->heads * (double)T * T * hd, 0,
-            attend(m, q, qd, k, kvd, v, kvd, att, qd, B, T, m->heads, m->kv_heads, hd, sshift, sq, mode, m->sliding, cs, sn, st,
-                   apl, apad, qd, &aflag));
+            attend(m, q, qd, k, kvd, v, kvd, att, qd, B, T, m->heads, m->kv_heads, hd, sshift, sq, mode, m->sliding, nullptr,
+                   nullptr, st, apl, apad, qd, &aflag));
         project_from(m, aflag ? apl : nullptr, aflag, att, qd, M, l.o, l.p_o, p, d, nullptr, 0, st);
         // p = post-attention norm(p) + x (p is the FFN's residual), xn = ffn_norm(p)
         if (nbuf && rms_pair(p, x, xn, l.post_attn, l.ffn_norm)) {
