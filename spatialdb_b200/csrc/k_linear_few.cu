@@ -10,7 +10,7 @@
 // cache in the same order. The tensor pipe is idle most of the time: what counts is the bytes in flight.
 // bf16 1 x 4096 x 11008: 16.5 us, 5455 GB/s; f16 8 x 4096 x 4096: 8.5 us; bf16 1 x 2048 x 16384 gated: 21.8 us,
 // 6148 GB/s.
-// f32, up to 8 rows: one block per 8 weight rows (4 + 4 when gated), four consecutive K values a lane,
+// f32, up to 16 rows: one block per 8 weight rows (4 + 4 when gated), four consecutive K values a lane,
 // fp32 FMAs. 1 x 4096 x 11008: 29.7 us, 6076 GB/s.
 // Both join the warps' partial sums in shared memory in a fixed order and apply the epilogue there.
 #include <algorithm>
@@ -35,7 +35,7 @@ struct FewParams {
     const void *x, *r;
     void* y;
     int64_t ldx, ldr, ldo, k4;
-    int M, N, K, nkb, act;
+    int M, N, K, nkb, act, parts;
 };
 
 template <class T>
@@ -165,13 +165,14 @@ __device__ __forceinline__ float4 load_x4(const FewParams& p, int m, int64_t k) 
     return v;
 }
 
-// MB: activation rows (1, 2, 4, 8).
+// MB: activation rows of a block (1, 2, 4, 8). More rows than that are shared by p.parts neighbouring blocks,
+// which read the same weights at about the same time (from L2, but for the first).
 template <int MB, bool GATED, bool VEC>
 __global__ void __launch_bounds__(FT, MB >= 4 ? 2 : 3) k_few32(FewParams p) {
     constexpr int S = GATED ? 2 : 1, R = 8 / S, NV = 8 * MB;  // weight rows a block, sums a lane
     __shared__ float red[WARPS][NV];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n0 = blockIdx.x * R;
+    const int n0 = (int)(blockIdx.x / p.parts) * R, m0 = (int)(blockIdx.x % p.parts) * MB, rows = min(p.M - m0, MB);
     const float* row[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -187,8 +188,8 @@ __global__ void __launch_bounds__(FT, MB >= 4 ? 2 : 3) k_few32(FewParams p) {
         for (int i = 0; i < 8; i++) w[i] = __ldg((const float4*)(row[i] + k));
 #pragma unroll
         for (int m = 0; m < MB; m++) {
-            if (m >= p.M) break;
-            const float4 x = load_x4<VEC>(p, m, k);
+            if (m >= rows) break;
+            const float4 x = load_x4<VEC>(p, m0 + m, k);
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 acc[i * MB + m] = fmaf(w[i].x, x.x, fmaf(w[i].y, x.y, fmaf(w[i].z, x.z, fmaf(w[i].w, x.w, acc[i * MB + m]))));
@@ -218,13 +219,13 @@ __global__ void __launch_bounds__(FT, MB >= 4 ? 2 : 3) k_few32(FewParams p) {
     __syncthreads();
     for (int o = threadIdx.x; o < R * MB; o += FT) {
         const int i = o / MB, m = o % MB, n = n0 + i;
-        if (m >= p.M || n >= p.N) continue;
+        if (m >= rows || n >= p.N) continue;
         float v[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < S; s++)
 #pragma unroll
             for (int q = 0; q < WARPS; q++) v[s] += red[q][(i + s * R) * MB + m];
-        finish<float>(p, m, n, v[0], v[1], GATED);
+        finish<float>(p, m0 + m, n, v[0], v[1], GATED);
     }
 }
 
@@ -235,21 +236,28 @@ void launch16(const FewParams& p, cudaStream_t st) {
     else k_few16<T, 2, GATED, VEC><<<grid, FT, 0, st>>>(p);
 }
 template <bool GATED, bool VEC>
-void launch32(const FewParams& p, cudaStream_t st) {
-    const unsigned grid = (unsigned)(GATED ? (p.N + 3) / 4 : (p.N + 7) / 8);
+void launch32(FewParams p, cudaStream_t st) {
+    // Up to eight rows to a block, four where eight would leave SMs without work (8 x 768 x 768: 4.0 and 3.2 us;
+    // 5 x 768 x 2304: 4.0 and 5.2).
+    const int64_t groups = GATED ? (p.N + 3) / 4 : (p.N + 7) / 8;
+    const int most = 2 * groups * ((p.M + 7) / 8) < 3 * device_sm_count() ? 4 : 8;
+    p.parts = (p.M + most - 1) / most;
+    const int mb = (p.M + p.parts - 1) / p.parts;
+    const unsigned grid = (unsigned)(groups * p.parts);
     if (p.M <= 1) k_few32<1, GATED, VEC><<<grid, FT, 0, st>>>(p);
     else if (p.M <= 2) k_few32<2, GATED, VEC><<<grid, FT, 0, st>>>(p);
-    else if (p.M <= 4) k_few32<4, GATED, VEC><<<grid, FT, 0, st>>>(p);
+    else if (mb <= 4) k_few32<4, GATED, VEC><<<grid, FT, 0, st>>>(p);
     else k_few32<8, GATED, VEC><<<grid, FT, 0, st>>>(p);
 }
 }  // namespace
 
 // f32 past 4 rows: the sums leave few registers for loads, and the tensor-core form, which reads six bytes a
-// weight instead of four, catches up from about 8 million weights on (8 rows, 4096 x 4096: 31.0 us here,
-// 25.9 there; 768 x 2304: 4.2 and 9.1).
+// weight instead of four, catches up (us here and there: 8 x 768 x 2304 4.2, 9.1; 8 x 4096 x 4096 30.8, 25.9;
+// 16 x 768 x 2304 7.8, 9.1; 10 x 8096 x 32 9.6, 24.8; 11 x 1632 x 10016 38.2, 36.2; 16 x 4096 x 4096 46.7, 25.9).
 bool few_supported(const Plan& p, int64_t M) {
-    if (p.dtype != DT_F32) return M <= 16;
-    return M <= 4 || (M <= 8 && (int64_t)p.N * p.K * (p.gated ? 2 : 1) <= (8 << 20));
+    if (p.dtype != DT_F32 || M <= 4) return M <= 16;
+    const int64_t weights = (int64_t)p.N * p.K * (p.gated ? 2 : 1);
+    return M <= 16 && weights <= (M <= 8 ? 8 << 20 : 4 << 20);
 }
 
 int few(const Plan& pl, const Call& c, cudaStream_t st) {
@@ -260,7 +268,7 @@ int few(const Plan& pl, const Call& c, cudaStream_t st) {
     p.bias = pl.bias; p.gbias = pl.gbias;
     p.x = c.x; p.r = c.r; p.y = c.y;
     p.ldx = c.ldx; p.ldr = c.ldr; p.ldo = c.ldo; p.k4 = pl.k4();
-    p.M = (int)c.M; p.N = pl.N; p.K = pl.K; p.nkb = pl.nkb(); p.act = pl.act;
+    p.M = (int)c.M; p.N = pl.N; p.K = pl.K; p.nkb = pl.nkb(); p.act = pl.act; p.parts = 1;
     const bool vec = (uintptr_t)c.x % 16 == 0 && (c.M == 1 || c.ldx % (f32 ? 4 : 8) == 0);
 #define SLX_PICK(fn, ...)                                                         \
     do {                                                                          \

@@ -312,22 +312,32 @@ __device__ __forceinline__ uint64_t operand(uint32_t start) {
     return d;
 }
 
-// Eight values of a row from column k, zeros past K: as few and wide loads as the address allows.
+// Eight values of a row from column k (a multiple of 8), zeros past K. Where they do not start on a 16-byte
+// boundary, the two aligned vectors around them, shifted together, while both lie inside the row (7 values
+// before, 8 behind); single values at the row's ends.
 __device__ __forceinline__ uint4 row8(const uint16_t* row, int k, int K) {
     const uint16_t* src = row + k;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (k + 8 <= K) {
-        if (((uintptr_t)src & 15) == 0) return *(const uint4*)src;
-        if (((uintptr_t)src & 3) == 0) {
-            const uint32_t* s4 = (const uint32_t*)src;
-            return make_uint4(s4[0], s4[1], s4[2], s4[3]);
-        }
+    const uint32_t off = (uint32_t)(uintptr_t)src & 15;
+    if (off == 0 && k + 8 <= K) return *(const uint4*)src;
+    if (k >= 8 && k + 16 <= K) {
+        const uint4* at = (const uint4*)((uintptr_t)src & ~(uintptr_t)15);
+        const uint4 lo = at[0], hi = at[1];
+        uint32_t w[7] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z};
+        const uint32_t last = hi.w;
+        // by two words, by one, by half of one
+        const bool two = off & 8, one = off & 4;
+        uint32_t t[6], u[5];
+#pragma unroll
+        for (int j = 0; j < 6; j++) t[j] = two ? (j + 2 < 7 ? w[j + 2] : last) : w[j];
+#pragma unroll
+        for (int j = 0; j < 5; j++) u[j] = one ? t[j + 1] : t[j];
+        const uint32_t bits = (off & 2) * 8;
+        return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits), __funnelshift_r(u[2], u[3], bits),
+                          __funnelshift_r(u[3], u[4], bits));
     }
     uint16_t e[8];
-    *(uint4*)e = v;
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        if (k + j < K) e[j] = src[j];
+    for (int j = 0; j < 8; j++) e[j] = k + j < K ? src[j] : (uint16_t)0;
     return *(const uint4*)e;
 }
 __device__ __forceinline__ void row8(const float* row, int k, int K, float (&f)[8]) {
@@ -954,7 +964,7 @@ void layout(const Plan& p, const void* w, uint8_t* tiles, float* rows, cudaStrea
 }
 
 // The form and tile of a call, by an estimate of its SM cycles. Fixed parts and rates as measured
-// (clock64 stamps in the kernel): about 3000 cycles from launch to the first MMA, a K block the larger
+// (clock64 stamps in the kernel, and every form and tile of 40 shapes timed): about 3000 cycles from launch to the first MMA, a K block the larger
 // of its MMAs (64 cycles each up to N = 128, N / 2 above) and its bytes at 56 a cycle, 1500 cycles for the
 // exchange in a cluster and 64 bytes a cycle stored in it, four outputs a cycle in the epilogue. Clusters of
 // 8 and 4 fit 15 and 33 times, pairs on all SMs.
@@ -976,7 +986,7 @@ Choice choose(const Plan& p, const Call& c) {
                 const double tiles = tiles_m * p.tiles_n();
                 const double waves = std::ceil(tiles / fit);
                 double block = std::max(S * steps * mma, (S * planes * TR * rowb + planes * nt * rowb) / 56.0);
-                if (pass) block = std::max(block, planes == 3 ? 1100.0 + 6.0 * nt : 500.0 + nt);
+                if (pass) block = std::max(block, planes == 3 ? 1100.0 + 6.0 * nt : 300.0 + 22.0 * nt);
                 const double t = waves * (3000 + std::ceil((double)p.nkb() / split) * block + out / split +
                                           (l ? 1500 + S * rows * TR * 4 / 64.0 : rows * TR * S * 4 / 256.0));
                 if (!best.nt || t < best.cycles) best = Choice{nt, ONE, l, t};

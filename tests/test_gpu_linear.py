@@ -156,7 +156,9 @@ def test_persistent_tiles(ctx, dtype, M, K, N):
 @pytest.mark.parametrize("dtype,M,K,N,gated,pad", [("f32", 20, 2048, 19000, False, 0), ("f32", 30, 1111, 19000, True, 1),
                                                    ("f32", 60, 1500, 19000, False, 0), ("f16", 31, 3001, 19000, False, 3),
                                                    ("bf16", 64, 2500, 19000, True, 1), ("bf16", 100, 4096, 18000, False, 0),
-                                                   ("f32", 7, 2100, 4100, False, 0), ("f32", 5, 2100, 2500, True, 2)])
+                                                   ("f32", 7, 2100, 4100, False, 0), ("f32", 5, 2100, 2500, True, 2),
+                                                   ("f32", 13, 300, 1111, False, 0), ("f32", 16, 513, 40, True, 1),
+                                                   ("bf16", 2100, 301, 200, False, 3), ("f16", 1500, 1111, 1300, True, 1)])
 def test_long_sums_of_one_tile(ctx, dtype, M, K, N, gated, pad):
     """So many weight tiles that none is split over K: one CTA goes through every K block, its stages many
     times over, and in f32 through many promotions, with its rows loaded by TMA and by the epilogue's warps."""
