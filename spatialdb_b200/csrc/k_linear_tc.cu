@@ -986,7 +986,7 @@ Choice choose(const Plan& p, const Call& c) {
                 const double tiles = tiles_m * p.tiles_n();
                 const double waves = std::ceil(tiles / fit);
                 double block = std::max(S * steps * mma, (S * planes * TR * rowb + planes * nt * rowb) / 56.0);
-                if (pass) block = std::max(block, planes == 3 ? 1100.0 + 6.0 * nt : 300.0 + 22.0 * nt);
+                if (pass) block = std::max(block, planes == 3 ? 1100.0 + 6.0 * nt : 200.0 + 22.0 * nt);
                 const double t = waves * (3000 + std::ceil((double)p.nkb() / split) * block + out / split +
                                           (l ? 1500 + S * rows * TR * 4 / 64.0 : rows * TR * S * 4 / 256.0));
                 if (!best.nt || t < best.cycles) best = Choice{nt, ONE, l, t};

@@ -306,15 +306,15 @@ int launch_float(const QkRope& p, cudaStream_t st) {
 
 // ---- Q30 -------------------------------------------------------------------------------------------
 
-// RmsNormRow's root for a head's wrapping sum of squares; skip: the row is left as it is (ms <= 0). A mean
-// square below 2^62 (values below 2 in Q30) takes 64-bit arithmetic: its quotient from a double estimate (off by
-// at most 2^10), corrected by the exact remainder, and its root from a double one, corrected by squaring.
-SLX_DEV int64_t q30_root(u128 ss, int n, bool& skip) {
+// RmsNormRow's root for a head's wrapping sum of squares, and its reciprocal; skip: the row is left as it is
+// (ms <= 0). A mean square below 2^62 (values below 2 in Q30) takes 64-bit arithmetic: its quotient from a double
+// estimate (off by at most 2^10), corrected by the exact remainder, and its root corrected by squaring. rn = 1 / n.
+SLX_DEV int64_t q30_root(u128 ss, int n, double rn, bool& skip, double& rd) {
     skip = (i128)ss < (i128)n;
+    rd = 1.0;
     if (skip) return 1;
     if ((ss >> 62) < (u128)(uint32_t)n) {
-        const double rn = 1.0 / (double)n;
-        const double sd = (double)(uint64_t)(ss >> 64) * 18446744073709551616.0 + (double)(uint64_t)ss;
+        const double sd = fma((double)(uint32_t)(ss >> 64), 18446744073709551616.0, (double)(uint64_t)ss);
         uint64_t ms = (uint64_t)(sd * rn);
         const int64_t rem = (int64_t)((uint64_t)ss - ms * (uint64_t)n);  // exact: the true value is small
         ms += (uint64_t)(int64_t)floor((double)rem * rn);
@@ -324,10 +324,13 @@ SLX_DEV int64_t q30_root(u128 ss, int n, bool& skip) {
         uint64_t r = (uint64_t)sqrt((double)ms);
         while (r * r > ms) r--;
         while ((r + 1) * (r + 1) <= ms) r++;
-        return r == 0 ? 1 : (int64_t)r;
+        rd = 1.0 / (double)r;
+        return (int64_t)r;
     }
-    const int64_t r = isqrt_u128(udiv128_u32(ss, (uint32_t)n, ~0ULL / (uint32_t)n));
-    return r == 0 ? 1 : r;
+    int64_t r = isqrt_u128(udiv128_u32(ss, (uint32_t)n, ~0ULL / (uint32_t)n));
+    if (r == 0) r = 1;
+    rd = 1.0 / (double)r;
+    return r;
 }
 
 // floor((a c - b s) / 2^30) and floor((a s + b c) / 2^30). With c, s a Q30 cosine and sine (c^2 + s^2 <= 2^60) and
@@ -364,9 +367,11 @@ SLX_DEV int64_t q30_scale(int64_t x, int64_t w, int64_t root, double rd) {
     return minus ? -q : q;
 }
 
-// One warp per head row, lane l owning the pairs l, l + 32, ... (PL of them, held in registers).
+// One warp per head row, lane l owning the pairs l, l + 32, ... (PL of them, held in registers). Bound by the
+// latency of a warp's chain (sum, root, exact quotients, rotation) at 32 warps an SM: four blocks (64 registers) of
+// 513 rows' 4617 warps run at once, 9.1 us; three (70 registers) take two waves, 12.2.
 template <int PL>
-__global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
+__global__ void __launch_bounds__(QT, PL <= 4 ? 4 : 2) k_qk_q30(QkRope p) {
     const int lane = threadIdx.x & 31, nheads = p.q.nh + p.k.nh;
     int64_t m;
     int head;
@@ -388,7 +393,7 @@ __global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
         a[e] = i < p.half ? x[i] : 0;
         b[e] = i < p.half ? x[i + p.half] : 0;
     }
-    bool skip = true, narrow = true;  // narrow: every |x| of the lane below 2^32, a square is one 32-bit product
+    bool skip = true, narrow = true;  // narrow: every |x| of the head below 2^32, a square is one 32-bit product
     int64_t root = 1;
     double rd = 1.0;
     if (w) {
@@ -400,13 +405,20 @@ __global__ void __launch_bounds__(QT) k_qk_q30(QkRope p) {
             ss += (u128)((uint64_t)(uint32_t)ua * (uint32_t)ua);
             ss += (u128)((uint64_t)(uint32_t)ub * (uint32_t)ub);
         }
-        if (!narrow) {
+        narrow = __all_sync(0xffffffffu, narrow);
+        if (narrow) {  // below 2^68 in a lane: three limbs of 27 bits, each summed over the lanes in one instruction
+            constexpr uint32_t MASK = (1u << 27) - 1;
+            const uint32_t l0 = __reduce_add_sync(0xffffffffu, (uint32_t)ss & MASK);
+            const uint32_t l1 = __reduce_add_sync(0xffffffffu, (uint32_t)(ss >> 27) & MASK);
+            const uint32_t l2 = __reduce_add_sync(0xffffffffu, (uint32_t)(ss >> 54));
+            ss = (u128)l0 + ((u128)l1 << 27) + ((u128)l2 << 54);
+        } else {
             ss = 0;
 #pragma unroll
             for (int e = 0; e < PL; e++) ss += (u128)((i128)a[e] * a[e]) + (u128)((i128)b[e] * b[e]);
+            ss = warp_sum_u128(ss);
         }
-        root = q30_root(warp_sum_u128(ss), p.hd, skip);
-        rd = 1.0 / (double)root;
+        root = q30_root(ss, p.hd, p.inv_hd, skip, rd);
     }
 #pragma unroll
     for (int e = 0; e < PL; e++) {
@@ -448,8 +460,7 @@ __global__ void __launch_bounds__(QT) k_qk_q30_wide(QkRope p) {
     if (w) {
         u128 ss = 0;
         for (int i = lane; i < p.hd; i += 32) ss += (u128)((i128)x[i] * x[i]);
-        root = q30_root(warp_sum_u128(ss), p.hd, skip);
-        rd = 1.0 / (double)root;
+        root = q30_root(warp_sum_u128(ss), p.hd, p.inv_hd, skip, rd);
     }
     for (int i = lane; i < p.half; i += 32) {
         int64_t u = x[i], v = x[i + p.half];
@@ -469,8 +480,10 @@ int qk_norm_rope(int dtype, const QkRope& p, cudaStream_t st) {
     return launch_float<float>(p, st);
 }
 
-int qk_norm_rope_q30(const QkRope& p, cudaStream_t st) {
+int qk_norm_rope_q30(const QkRope& given, cudaStream_t st) {
+    QkRope p = given;
     if (p.M <= 0 || p.q.nh + p.k.nh <= 0) return 0;
+    p.inv_hd = 1.0 / (double)p.hd;
     const int64_t units = p.M * (p.q.nh + p.k.nh);
     const unsigned grid = (unsigned)((units + QT / 32 - 1) / (QT / 32));
     if (p.half <= 32) k_qk_q30<1><<<grid, QT, 0, st>>>(p);

@@ -29,6 +29,7 @@ struct QkRope {
     const float2* table = nullptr;                       // float: (cos, sin) [table_rows][half]
     const int64_t *cs = nullptr, *sn = nullptr;          // Q30: [table_rows][half]
     float eps = 0.0f;
+    double inv_hd = 0.0;           // 1 / hd, set by the Q30 launcher
     int* err = nullptr;            // context error word: KERR_RANGE for a position outside the table
 };
 
