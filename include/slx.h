@@ -218,7 +218,7 @@ slx_status slx_attention(slx_ctx* ctx, const int64_t* q, const int64_t* k, const
  * y = act(x . gate^T + gate_bias) * (x . w^T + bias) + residual (the gated FFN's first half).
  * slx_linear_prepare lays the weights out once, on the context's stream, and waits: the buffers at d_w,
  * d_gate, d_bias and d_gate_bias (device memory, complete before the call; the biases f32[N], nullable)
- * may be freed afterwards. dtype is the type of x,
+ * may be freed afterwards; the handle itself must outlive graphs that captured its calls. dtype is the type of x,
  * residual and y: F32 takes weights of any GGUF type slx_dequantize decodes, F16 and BF16 weights of their
  * own type. d_gate NULL: no gate. Sums and the epilogue are fp32, rounded once to dtype.
  * An F32 product of more than 8 rows runs on the tensor cores from three bf16 parts of every value: a

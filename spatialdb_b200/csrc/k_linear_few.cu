@@ -63,7 +63,7 @@ __device__ __forceinline__ uint4 load_x8(const FewParams& p, int m, int k) {
     if (m >= p.M || k >= p.K) return v;
     const T* x = (const T*)p.x + (int64_t)m * p.ldx + k;
     if (VEC && k + 8 <= p.K) return *(const uint4*)x;
-    T e[8];
+    alignas(16) T e[8];
     *(uint4*)e = v;
 #pragma unroll
     for (int i = 0; i < 8; i++)
@@ -107,11 +107,12 @@ __global__ void __launch_bounds__(FT) k_few16(FewParams p) {
             const bool live = kb < p.nkb;
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                const uint8_t* q = src[s] + (int64_t)(live ? kb : kb0) * TR * 128;  // past the end: a block once more, times zeros
-                w[u][s][0] = __ldg((const uint4*)(q + off));
-                w[u][s][1] = __ldg((const uint4*)(q + off + 1024));
-                w[u][s][2] = __ldg((const uint4*)(q + (off ^ 64)));
-                w[u][s][3] = __ldg((const uint4*)(q + (off ^ 64) + 1024));
+                const uint8_t* q = src[s] + (int64_t)kb * TR * 128;
+                const uint4 none = make_uint4(0, 0, 0, 0);
+                w[u][s][0] = live ? __ldg((const uint4*)(q + off)) : none;
+                w[u][s][1] = live ? __ldg((const uint4*)(q + off + 1024)) : none;
+                w[u][s][2] = live ? __ldg((const uint4*)(q + (off ^ 64))) : none;
+                w[u][s][3] = live ? __ldg((const uint4*)(q + (off ^ 64) + 1024)) : none;
             }
 #pragma unroll
             for (int i = 0; i < MT; i++)

@@ -185,7 +185,7 @@ struct Columns {
         for (int j = 0; j < 8; j++) v[j] = from && at(j) < N ? from[at(j)] : 0.0f;
     }
 
-    struct Four {
+    struct __align__(4 * sizeof(T)) Four {
         T v[4];
     };
     struct __align__(16) Residual {
@@ -335,7 +335,7 @@ __device__ __forceinline__ uint4 row8(const uint16_t* row, int k, int K) {
         return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits), __funnelshift_r(u[2], u[3], bits),
                           __funnelshift_r(u[3], u[4], bits));
     }
-    uint16_t e[8];
+    alignas(16) uint16_t e[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) e[j] = k + j < K ? src[j] : (uint16_t)0;
     return *(const uint4*)e;
@@ -366,7 +366,7 @@ struct Chunk {
 };
 template <>
 struct Chunk<3> {
-    float f[8];
+    alignas(16) float f[8];
     __device__ __forceinline__ void load(const TcParams& p, int64_t m, int k) {
         if (m < p.M) {
             row8((const float*)p.x + m * p.ldx, k, p.K, f);
@@ -529,10 +529,10 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                 }
             }
             if (!ok) {  // let copies still in flight land before the CTA exits (they always complete)
-                if (MODE != PAIR) {
+                if (MODE != PAIR && !MANUAL) {
                     for (int j = done - ST < 0 ? 0 : done - ST; j < done; j++)
                         mbar_wait(full0 + 8 * (j % ST), (uint32_t)(j / ST) & 1u);
-                } else {  // counted on the leader's barriers, whose phases may stay open: a millisecond instead
+                } else {  // their barriers also count the other CTA's copies, or rows that may not come: a millisecond
                     const long long t0 = clock64();
                     while (clock64() - t0 < 2000000) __nanosleep(1000);
                 }
@@ -695,7 +695,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                     }
                     if (PLANES == 1 && c + SLAB == HC) release(buf);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                    float v[8 * R], g[8 * R];
+                    alignas(16) float v[8 * R], g[8 * R];
 #pragma unroll
                     for (int i = 0; i < 2 * R; i++) {
                         *(float4*)(v + 4 * i) = *(const float4*)(src + (i >> 1) * 8 * TR + (i & 1) * 64);
@@ -784,7 +784,7 @@ __global__ void k_tiles16(const uint16_t* __restrict__ w, int N, int K, int nkb,
         const int64_t blk = i >> 10;  // tile * nkb + kb
         const int64_t n = blk / nkb * TR + row;
         const int k = (int)(blk % nkb) * 64 + c * 8;
-        uint16_t e[8];
+        alignas(16) uint16_t e[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) e[j] = n < N && k + j < K ? w[n * K + k + j] : (uint16_t)0;
         out[(i & ~(int64_t)7) | (c ^ (row & 7))] = *(const uint4*)e;
@@ -821,7 +821,7 @@ __global__ void k_split_x(const float* __restrict__ x, int64_t ldx, int64_t M, i
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t m = i / (kp / 8);
         const int k = (int)(i % (kp / 8)) * 8;
-        float f[8];
+        alignas(16) float f[8];
         row8(x + m * ldx, k, K, f);
         uint4 part[3];
         split3(f, part);

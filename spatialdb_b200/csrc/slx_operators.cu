@@ -1,7 +1,9 @@
 // slx_operators.cu -- C ABI of the float linear operator and of the fused query/key norm and rotation.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <memory>
+#include <new>
 #include <vector>
 
 #include <cuda_runtime.h>
@@ -36,19 +38,18 @@ struct OnDevice {
 bool is_float(int dtype) { return dtype == SLX_DTYPE_F32 || dtype == SLX_DTYPE_F16 || dtype == SLX_DTYPE_BF16; }
 int width_of(int dtype) { return dtype == SLX_DTYPE_F32 ? 4 : dtype == SLX_DTYPE_Q30 ? 8 : 2; }
 
-// Stream-ordered scratch of one call: every call has its own, so calls on several streams and captured
-// graphs (whose allocations belong to the graph) never share it. The pool keeps what it has freed.
-int scratch(slx_ctx* ctx, size_t bytes, cudaStream_t st, void** p) {
-    if (!ctx->pool) {
-        cudaMemPoolProps props = {};
-        props.allocType = cudaMemAllocationTypePinned;
-        props.location.type = cudaMemLocationTypeDevice;
-        props.location.id = ctx->device;
-        CK(cudaMemPoolCreate(&ctx->pool, &props));
-        uint64_t keep = ~0ull;
-        CK(cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep));
-    }
-    CK(cudaMallocFromPoolAsync(p, bytes, ctx->pool, st));
+// The pool of the calls' stream-ordered scratch, made with the first operator (a call may be in a capture).
+// Every call has its own allocation, so calls on several streams and captured graphs (whose allocations belong
+// to the graph) never share one. The pool keeps what is freed.
+int ensure_pool(slx_ctx* ctx) {
+    if (ctx->pool) return SLX_OK;
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = ctx->device;
+    CK(cudaMemPoolCreate(&ctx->pool, &props));
+    uint64_t keep = ~0ull;
+    CK(cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep));
     return SLX_OK;
 }
 
@@ -66,7 +67,7 @@ struct slx_linear {
 
 struct slx_rope {
     slx_ctx* ctx = nullptr;
-    int refs = 1;  // slx_rope_free's reference plus one per slx_qk_norm
+    std::atomic<int> refs{1};  // slx_rope_free's reference plus one per slx_qk_norm
     int rows = 0, rot = 0, q30 = 0;
     float2* table = nullptr;
     int64_t *cs = nullptr, *sn = nullptr;
@@ -92,7 +93,7 @@ struct slx_qk_norm {
 namespace {
 
 void rope_release(slx_rope* r) {
-    if (--r->refs > 0) return;
+    if (r->refs.fetch_sub(1) != 1) return;
     slx_ctx* ctx = r->ctx;
     delete r;
     ctx_release(ctx);
@@ -174,6 +175,7 @@ slx_status slx_linear_prepare(slx_ctx* ctx, int dtype, const uint8_t* d_w, int64
     if (((uintptr_t)d_bias | (uintptr_t)d_gate_bias) % 4) return set_err(ctx, SLX_EINVAL, "bias not aligned to 4 bytes");
     OnDevice on(ctx->device);
     CK(on.err);
+    if (int rc = ensure_pool(ctx)) return rc;
     std::unique_ptr<slx_linear> h(new slx_linear());
     h->ctx = ctx;
     lin::Plan& p = h->plan;
@@ -241,7 +243,7 @@ slx_status slx_linear_device(slx_linear* l, const slx_linear_args* a) {
     const lin::Choice ch = lin::choose(p, c);
     void* ws = nullptr;
     if (const size_t need = lin::tc_workspace(p, c, ch)) {
-        if (int rc = scratch(ctx, need, st, &ws)) return rc;
+        CK(cudaMallocFromPoolAsync(&ws, need, ctx->pool, st));
     }
     int n = 0;
     run_k(ctx, KC_GEMM, macs, bytes, st, [&] { return (n = lin::tc(p, c, ch, ws, st)) < 0 ? 0 : n; });
@@ -259,32 +261,41 @@ slx_status slx_rope_create(slx_ctx* ctx, int rows, int rot_dim, float base, int 
     *out = nullptr;
     if (rows <= 0 || rot_dim <= 0 || rot_dim % 2 || rot_dim > 65536 || !(base > 0.0f) || !std::isfinite(base))
         return set_err(ctx, SLX_EINVAL, "bad rotation table: %d rows, width %d, base %g", rows, rot_dim, (double)base);
+    if ((int64_t)rows * (rot_dim / 2) > (1 << 28))
+        return set_err(ctx, SLX_EINVAL, "rotation table of %d rows x %d: more than 2^28 entries", rows, rot_dim / 2);
     OnDevice on(ctx->device);
     CK(on.err);
-    std::unique_ptr<slx_rope> r(new slx_rope());
-    r->ctx = ctx;
-    r->rows = rows; r->rot = rot_dim; r->q30 = q30 ? 1 : 0;
-    const int half = rot_dim / 2;
-    const size_t n = (size_t)rows * half;
-    if (q30) {
-        std::vector<int64_t> cs, sn;
-        rope_table(rows, rot_dim, base, cs, sn);
-        CK(cudaMalloc(&r->cs, n * 8));
-        CK(cudaMalloc(&r->sn, n * 8));
-        CK(cudaMemcpy(r->cs, cs.data(), n * 8, cudaMemcpyHostToDevice));
-        CK(cudaMemcpy(r->sn, sn.data(), n * 8, cudaMemcpyHostToDevice));
-    } else {
-        // Angles in double, each entry rounded to fp32 once: far positions keep their angle.
-        std::vector<double> theta((size_t)half);
-        for (int i = 0; i < half; i++) theta[i] = std::pow((double)base, -2.0 * i / rot_dim);
-        std::vector<float2> t(n);
-        for (int m = 0; m < rows; m++)
-            for (int i = 0; i < half; i++) {
-                const double a = m * theta[i];
-                t[(size_t)m * half + i] = make_float2((float)std::cos(a), (float)std::sin(a));
-            }
-        CK(cudaMalloc(&r->table, n * sizeof(float2)));
-        CK(cudaMemcpy(r->table, t.data(), n * sizeof(float2), cudaMemcpyHostToDevice));
+    std::unique_ptr<slx_rope> r;
+    try {
+        r.reset(new slx_rope());
+        r->ctx = ctx;
+        r->rows = rows; r->rot = rot_dim; r->q30 = q30 ? 1 : 0;
+        const int half = rot_dim / 2;
+        const size_t n = (size_t)rows * half;
+        if (q30) {
+            std::vector<int64_t> cs, sn;
+            rope_table(rows, rot_dim, base, cs, sn);
+            CK(cudaMalloc(&r->cs, n * 8));
+            CK(cudaMalloc(&r->sn, n * 8));
+            CK(cudaMemcpyAsync(r->cs, cs.data(), n * 8, cudaMemcpyHostToDevice, ctx->stream));
+            CK(cudaMemcpyAsync(r->sn, sn.data(), n * 8, cudaMemcpyHostToDevice, ctx->stream));
+            CK(cudaStreamSynchronize(ctx->stream));
+        } else {
+            // Angles in double, each entry rounded to fp32 once: far positions keep their angle.
+            std::vector<double> theta((size_t)half);
+            for (int i = 0; i < half; i++) theta[i] = std::pow((double)base, -2.0 * i / rot_dim);
+            std::vector<float2> t(n);
+            for (int m = 0; m < rows; m++)
+                for (int i = 0; i < half; i++) {
+                    const double a = m * theta[i];
+                    t[(size_t)m * half + i] = make_float2((float)std::cos(a), (float)std::sin(a));
+                }
+            CK(cudaMalloc(&r->table, n * sizeof(float2)));
+            CK(cudaMemcpyAsync(r->table, t.data(), n * sizeof(float2), cudaMemcpyHostToDevice, ctx->stream));
+            CK(cudaStreamSynchronize(ctx->stream));
+        }
+    } catch (const std::bad_alloc&) {
+        return set_err(ctx, SLX_EOOM, "host memory for a rotation table of %d rows", rows);
     }
     ctx->refs.fetch_add(1);
     *out = r.release();
@@ -323,7 +334,7 @@ slx_status slx_qk_norm_prepare(slx_rope* r, int dtype, int heads, int kv_heads, 
     if (int st = copy_vector(ctx, d_wq, (size_t)e * head_dim, &h->wq)) return st;
     if (int st = copy_vector(ctx, d_wk, (size_t)e * head_dim, &h->wk)) return st;
     h->rope = r;
-    r->refs++;
+    r->refs.fetch_add(1);
     ctx->refs.fetch_add(1);
     *out = h.release();
     return SLX_OK;
@@ -361,7 +372,7 @@ slx_status slx_qk_norm_rope_device(slx_qk_norm* h, const slx_qk_args* a) {
     if (!a->pos && T <= 0) return set_err(ctx, SLX_EINVAL, "sequence length %lld", (long long)T);
     if (!a->pos && std::min(T, M) > r->rows)
         return set_err(ctx, SLX_ERANGE, "sequence length %lld exceeds the RoPE table (%d rows)", (long long)T, r->rows);
-    if (M > (1ll << 33) / (h->heads + h->kv_heads))
+    if (M > (1ll << 32) / (h->heads + h->kv_heads))
         return set_err(ctx, SLX_EINVAL, "M %lld rows of %d heads", (long long)M, h->heads + h->kv_heads);
     OnDevice on(ctx->device);
     CK(on.err);

@@ -117,7 +117,7 @@ class Case:
 SIZES = [(1, 1, 1), (1, 7, 5), (1, 768, 768), (2, 64, 16), (3, 65, 17), (4, 200, 129), (5, 1000, 40), (8, 256, 300), (9, 96, 128),
          (15, 1001, 33), (16, 512, 1000), (17, 31, 128), (17, 32, 1), (24, 2048, 130), (32, 64, 640), (33, 640, 256),
          (40, 1001, 1111), (64, 1024, 128), (65, 33, 257), (100, 300, 300), (128, 4096, 136), (129, 257, 127), (200, 512, 200),
-         (257, 96, 3000), (300, 768, 768)]
+         (257, 96, 3000), (300, 768, 768), (20, 1, 5), (200, 3, 300), (3000, 2, 700)]
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
@@ -257,8 +257,8 @@ def test_gguf_weights_under_f32(ctx, oracle, wdtype, M):
 def test_streams_and_graphs(ctx):
     """Calls on two streams at once, and two captured graphs whose calls need scratch (f32, and rows TMA
     cannot address), replayed together with an eager call between them: nothing is shared."""
-    cases = [Case(ctx, "f32", 300, 512, 400, bias=True), Case(ctx, "f32", 200, 384, 300, residual=True),
-             Case(ctx, "bf16", 130, 257, 200, pad=3), Case(ctx, "f16", 4, 512, 300, bias=True)]
+    cases = [Case(ctx, "f32", 3000, 512, 1000, bias=True), Case(ctx, "f32", 200, 384, 300, residual=True),
+             Case(ctx, "bf16", 3000, 257, 600, pad=3), Case(ctx, "f16", 4, 512, 300, bias=True)]
     firsts = [c.run().clone() for c in cases]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in cases]
@@ -287,11 +287,45 @@ def test_streams_and_graphs(ctx):
             assert torch.equal(c.y[:, : c.N], f)
 
 
+def test_first_call_inside_a_capture():
+    """A context whose first calls are captured: nothing they need is made inside the capture."""
+    own = slx.Context(0)
+    cases = [Case(own, "f32", 2500, 320, 900), Case(own, "f16", 1700, 333, 800, pad=1), Case(own, "bf16", 50, 96, 70)]
+    s = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        for c in cases:
+            c.run(stream=s.cuda_stream)
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        for c in cases:
+            c.check(got=c.y[:, : c.N])
+            c.y.fill_(7)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M", [1, 12, 40])
+def test_infinite_weights(ctx, dtype, M):
+    """An infinite weight makes its own output infinite where x is not zero, whatever the padding around it."""
+    c = Case(ctx, dtype, M, 70, 20)
+    c.x.abs_().add_(0.5)
+    w = c.w.clone()
+    w[7, 3] = float("inf")
+    torch.cuda.synchronize()
+    op = slx.Linear(c.code, w.data_ptr(), w.numel() * 2, c.code, 20, 70, ctx=ctx)
+    op.apply_device(c.x.data_ptr(), M, c.y.data_ptr(), ldx=c.x.stride(0), stream=slx.STREAM_LEGACY)
+    torch.cuda.synchronize()
+    assert bool((c.y[:, 7] == float("inf")).all()) and bool(c.y[:, torch.arange(20) != 7].isfinite().all())
+
+
 def test_wait_that_gives_up_is_reported():
     """The tensor-core kernel's bounded waits: with its MMA warp idle and a short limit the call ends,
     the status is reported once, and the context computes the next call."""
     own = slx.Context(0)
-    for dtype, M, N in (("bf16", 40, 128), ("f32", 300, 6000), ("bf16", 2000, 3000)):  # split and persistent
+    # one tile a cluster (rows by TMA, by the epilogue's warps) and pairs
+    for dtype, M, N in (("bf16", 40, 128), ("f32", 40, 256), ("f32", 3000, 2000), ("bf16", 2000, 3000)):
         c = Case(own, dtype, M, 512, N)
         own.set_option(slx.OPT_WAIT_LIMIT_CYCLES, 2_000_000)
         own.set_option(slx.OPT_TEST_STALL_MMA, 1)

@@ -235,7 +235,8 @@ def test_refusals(ctx):
             fn(*a, **k)
         assert e.value.status == status
 
-    for a in ((0, 64), (10, 0), (10, 63), (10, 64, 0.0), (10, 64, float("inf")), (10, 64, -1.0)):
+    for a in ((0, 64), (10, 0), (10, 63), (10, 64, 0.0), (10, 64, float("inf")), (10, 64, -1.0),
+              (2 ** 31 - 1, 65536)):
         refused(slx.SLX_EINVAL, slx.RopeTable, *a, ctx=ctx)
     t, ti = slx.RopeTable(32, 64, ctx=ctx), slx.RopeTable(32, 64, q30=True, ctx=ctx)
     w = torch.ones(64, device="cuda")
