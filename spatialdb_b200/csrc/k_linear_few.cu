@@ -98,15 +98,16 @@ __global__ void __launch_bounds__(FT) k_few16(FewParams p) {
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[s][i][j] = 0.0f;
+    grid_wait();
     for (int kb0 = warp; kb0 < p.nkb; kb0 += WARPS * U) {
         // everything the U blocks need is asked for before any of it is used
-        uint4 w[U][S][4], x[U][MT][2];
+        uint4 w[U][S][4];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int kb = kb0 + u * WARPS;
-            const bool live = kb < p.nkb;
+        for (int u = 0; u < U; u++)
 #pragma unroll
             for (int s = 0; s < S; s++) {
+                const int kb = kb0 + u * WARPS;
+                const bool live = kb < p.nkb;
                 const uint8_t* q = src[s] + (int64_t)kb * TR * 128;
                 const uint4 none = make_uint4(0, 0, 0, 0);
                 w[u][s][0] = live ? __ldg((const uint4*)(q + off)) : none;
@@ -114,11 +115,16 @@ __global__ void __launch_bounds__(FT) k_few16(FewParams p) {
                 w[u][s][2] = live ? __ldg((const uint4*)(q + (off ^ 64))) : none;
                 w[u][s][3] = live ? __ldg((const uint4*)(q + (off ^ 64) + 1024)) : none;
             }
+        uint4 x[U][MT][2];
+#pragma unroll
+        for (int u = 0; u < U; u++)
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int c = 0; c < 2; c++) x[u][i][c] = load_x8<T, VEC>(p, live ? g + 8 * i : p.M, kb * 64 + c * 32 + t * 8);
-        }
+                for (int c = 0; c < 2; c++) {
+                    const int kb = kb0 + u * WARPS;
+                    x[u][i][c] = load_x8<T, VEC>(p, kb < p.nkb ? g + 8 * i : p.M, kb * 64 + c * 32 + t * 8);
+                }
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -132,6 +138,7 @@ __global__ void __launch_bounds__(FT) k_few16(FewParams p) {
                         mma16816<T>(acc[s][i], lo.z, hi.z, lo.w, hi.w, v.z, v.w);
                     }
     }
+    grid_release();  // not earlier: the next kernel's blocks would share the memory's rate with this one's
 #pragma unroll
     for (int s = 0; s < S; s++)
 #pragma unroll
@@ -183,10 +190,17 @@ __global__ void __launch_bounds__(FT, MB >= 4 ? 2 : 3) k_few32(FewParams p) {
     float acc[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) acc[i] = 0.0f;
-    for (int64_t k = (int64_t)threadIdx.x * 4; k < p.k4; k += FT * 4) {
-        float4 w[8];
+    grid_release();
+    float4 w[8];
+    auto weights = [&](int64_t k) {
 #pragma unroll
         for (int i = 0; i < 8; i++) w[i] = __ldg((const float4*)(row[i] + k));
+    };
+    const int64_t k0 = (int64_t)threadIdx.x * 4;
+    if (k0 < p.k4) weights(k0);  // the handle's own memory: no kernel in the stream writes it
+    grid_wait();
+    for (int64_t k = k0; k < p.k4; k += FT * 4) {
+        if (k != k0) weights(k);
 #pragma unroll
         for (int m = 0; m < MB; m++) {
             if (m >= rows) break;
@@ -233,8 +247,8 @@ __global__ void __launch_bounds__(FT, MB >= 4 ? 2 : 3) k_few32(FewParams p) {
 template <class T, bool GATED, bool VEC>
 void launch16(const FewParams& p, cudaStream_t st) {
     const unsigned grid = (unsigned)((p.N + 15) / 16);
-    if (p.M <= 8) k_few16<T, 1, GATED, VEC><<<grid, FT, 0, st>>>(p);
-    else k_few16<T, 2, GATED, VEC><<<grid, FT, 0, st>>>(p);
+    if (p.M <= 8) launch_early(k_few16<T, 1, GATED, VEC>, grid, FT, 0, st, 1, p);
+    else launch_early(k_few16<T, 2, GATED, VEC>, grid, FT, 0, st, 1, p);
 }
 template <bool GATED, bool VEC>
 void launch32(FewParams p, cudaStream_t st) {
@@ -245,10 +259,10 @@ void launch32(FewParams p, cudaStream_t st) {
     p.parts = (p.M + most - 1) / most;
     const int mb = (p.M + p.parts - 1) / p.parts;
     const unsigned grid = (unsigned)(groups * p.parts);
-    if (p.M <= 1) k_few32<1, GATED, VEC><<<grid, FT, 0, st>>>(p);
-    else if (p.M <= 2) k_few32<2, GATED, VEC><<<grid, FT, 0, st>>>(p);
-    else if (mb <= 4) k_few32<4, GATED, VEC><<<grid, FT, 0, st>>>(p);
-    else k_few32<8, GATED, VEC><<<grid, FT, 0, st>>>(p);
+    if (p.M <= 1) launch_early(k_few32<1, GATED, VEC>, grid, FT, 0, st, 1, p);
+    else if (p.M <= 2) launch_early(k_few32<2, GATED, VEC>, grid, FT, 0, st, 1, p);
+    else if (mb <= 4) launch_early(k_few32<4, GATED, VEC>, grid, FT, 0, st, 1, p);
+    else launch_early(k_few32<8, GATED, VEC>, grid, FT, 0, st, 1, p);
 }
 }  // namespace
 

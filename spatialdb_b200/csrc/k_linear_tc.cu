@@ -453,6 +453,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     uint32_t* tmem_slot = (uint32_t*)(bars + 2 * ST + 5);
     __shared__ int s_fail;
 
+    grid_release();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long limit = p.wait_limit;
     if (threadIdx.x == 0) {
@@ -497,6 +498,20 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
 
     if (warp == 0) {
         if (lane == 0) {  // producer, running ahead across tiles
+            auto load_w = [&](int kb, int stage, int64_t blk0) {
+                const uint32_t dst = sbase + stage * Sh::STAGE, bar = full0 + 8 * stage;
+                if (MODE == PAIR) {
+                    const uint32_t lead = peer_addr(bar, 0);
+                    if (rank == 0) mbar_expect_tx(bar, 2 * Sh::STAGE);
+                    const int line = (int)((blk0 + kb) * (Sh::WB / 128));
+                    pair_load_2d(dst, &tmw, 0, line, lead);
+                    if (GATED) pair_load_2d(dst + Sh::WB, &tmg, 0, line, lead);
+                } else {
+                    mbar_expect_tx(bar, MANUAL ? S * Sh::WB : Sh::STAGE);
+                    bulk_load(dst, p.w + (blk0 + kb) * Sh::WB, Sh::WB, bar);
+                    if (GATED) bulk_load(dst + Sh::WB, p.g + (blk0 + kb) * Sh::WB, Sh::WB, bar);
+                }
+            };
             int done = 0, s = 0;
             uint32_t ph = 0;
             bool ok = true;
@@ -505,26 +520,22 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                 tile_at(p, tiles_n, t, tm, tn);
                 const int m0 = tm * NT + (MODE == PAIR ? rank * Sh::XR : 0);
                 const int64_t blk0 = (int64_t)(MODE == PAIR ? 2 * tn + rank : tn) * p.nkb;
+                // Weights are the handle's own memory, which no kernel in the stream writes: the first stages' are
+                // asked for before the kernels ahead of this one are waited for, the activations after it.
+                const int ahead = MODE == ONE ? (kb1 - kb0 < ST ? kb1 - kb0 : ST) : 0;
+                for (int i = 0; i < ahead; i++) load_w(kb0 + i, i, blk0);
+                if (done == 0) grid_wait();
                 for (int kb = kb0; kb < kb1; kb++, done++) {
-                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1u, limit) || *(volatile int*)&s_fail) {
+                    const bool asked = done < ahead;
+                    if (!asked && (!mbar_wait(empty0 + 8 * s, ph ^ 1u, limit) || *(volatile int*)&s_fail)) {
                         s_fail = 1;
                         ok = false;
                         break;
                     }
-                    const uint32_t dst = sbase + s * Sh::STAGE, bar = full0 + 8 * s;
-                    if (MODE == PAIR) {
-                        const uint32_t lead = peer_addr(bar, 0);
-                        if (rank == 0) mbar_expect_tx(bar, 2 * Sh::STAGE);
-                        const int line = (int)((blk0 + kb) * (Sh::WB / 128));
-                        pair_load_2d(dst, &tmw, 0, line, lead);
-                        if (GATED) pair_load_2d(dst + Sh::WB, &tmg, 0, line, lead);
-                        pair_load_3d(dst + S * Sh::WB, &tmx, kb * (ROWB / 2), m0, 0, lead);
-                    } else {
-                        mbar_expect_tx(bar, MANUAL ? S * Sh::WB : Sh::STAGE);
-                        bulk_load(dst, p.w + (blk0 + kb) * Sh::WB, Sh::WB, bar);
-                        if (GATED) bulk_load(dst + Sh::WB, p.g + (blk0 + kb) * Sh::WB, Sh::WB, bar);
-                        if (!MANUAL) tma_load_3d(dst + S * Sh::WB, &tmx, kb * (ROWB / 2), m0, 0, bar);
-                    }
+                    if (!asked) load_w(kb, s, blk0);
+                    const uint32_t dst = sbase + s * Sh::STAGE + S * Sh::WB, bar = full0 + 8 * s;
+                    if (MODE == PAIR) pair_load_3d(dst, &tmx, kb * (ROWB / 2), m0, 0, peer_addr(bar, 0));
+                    else if (!MANUAL) tma_load_3d(dst, &tmx, kb * (ROWB / 2), m0, 0, bar);
                     if (++s == ST) { s = 0; ph ^= 1u; }
                 }
             }
@@ -601,6 +612,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
         float* st = out_stage + part * S * SLAB * TR;
         const int tid = (int)threadIdx.x - 64 - 128 * part, col = tid >> 4;
         const float* src = st + col * TR + (tid & 15) * 4;
+        grid_wait();  // x, the residual and y belong to the kernels ahead until they have ended
         int use = 0;
         auto release = [&](int buf) {  // this warp has read the buffer
             fence_before();
@@ -905,20 +917,7 @@ bool launch(const Plan& pl, const Call& c, const Operands& op, int log2_split, c
         grid = 2 * std::min(p.tiles, n);
     }
     const int size = MODE == PAIR ? 2 : 1 << log2_split;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(LT);
-    cfg.dynamicSmemBytes = Sh::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    if (size > 1) {
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = (unsigned)size;
-        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-    }
-    return cudaLaunchKernelEx(&cfg, fn, tmx, tmw, tmg, p) == cudaSuccess;
+    return launch_early(fn, dim3((unsigned)grid), dim3(LT), Sh::SMEM, st, size, tmx, tmw, tmg, p) == cudaSuccess;
 }
 
 bool tma_rows(const Plan& p, const Call& c) {  // the caller's 16-bit rows as they are

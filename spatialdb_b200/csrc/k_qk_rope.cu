@@ -143,6 +143,8 @@ __global__ void __launch_bounds__(QV) k_qk_vec(QkRope p, Slabs sl) {
     int64_t m;
     int slab;
     divide((int64_t)blockIdx.x * (QV / 32) + (threadIdx.x >> 5), sl.q + sl.k, p.M * (sl.q + sl.k) + QV, m, slab);
+    grid_release();
+    grid_wait();
     if (m >= p.M) return;
     const bool isq = slab < sl.q;
     const QkSide& s = isq ? p.q : p.k;
@@ -230,6 +232,8 @@ __global__ void __launch_bounds__(QT) k_qk_any(QkRope p) {
     int64_t m;
     int head;
     divide((int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5), nheads, p.M * nheads + QT, m, head);
+    grid_release();
+    grid_wait();
     if (m >= p.M) return;
     const int pos = position(p, m);
     if (pos < 0) return;
@@ -271,7 +275,7 @@ int launch_steps(const QkRope& p, cudaStream_t st) {
     const int heads = 32 / G * STEPS;  // of a warp
     const Slabs sl{(p.q.nh + heads - 1) / heads, (p.k.nh + heads - 1) / heads};
     const int64_t units = p.M * (sl.q + sl.k);
-    k_qk_vec<T, G, STEPS><<<(unsigned)((units + QV / 32 - 1) / (QV / 32)), QV, 0, st>>>(p, sl);
+    launch_early(k_qk_vec<T, G, STEPS>, (unsigned)((units + QV / 32 - 1) / (QV / 32)), QV, 0, st, 1, p, sl);
     return 1;
 }
 // One step to a warp while that leaves SMs without work (the least latency), then two and four (f16 3001 x (20 + 4) x
@@ -300,7 +304,7 @@ int launch_float(const QkRope& p, cudaStream_t st) {
         return launch_vec<T, 32>(p, st);
     }
     const int64_t units = p.M * (p.q.nh + p.k.nh);
-    k_qk_any<T><<<(unsigned)((units + QT / 32 - 1) / (QT / 32)), QT, 0, st>>>(p);
+    launch_early(k_qk_any<T>, (unsigned)((units + QT / 32 - 1) / (QT / 32)), QT, 0, st, 1, p);
     return 1;
 }
 
@@ -376,6 +380,8 @@ __global__ void __launch_bounds__(QT, PL <= 4 ? 4 : 2) k_qk_q30(QkRope p) {
     int64_t m;
     int head;
     divide((int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5), nheads, p.M * nheads + QT, m, head);
+    grid_release();
+    grid_wait();
     if (m >= p.M) return;
     const int pos = position(p, m);
     if (pos < 0) return;
@@ -445,6 +451,8 @@ __global__ void __launch_bounds__(QT) k_qk_q30_wide(QkRope p) {
     int64_t m;
     int head;
     divide((int64_t)blockIdx.x * (QT / 32) + (threadIdx.x >> 5), nheads, p.M * nheads + QT, m, head);
+    grid_release();
+    grid_wait();
     if (m >= p.M) return;
     const int pos = position(p, m);
     if (pos < 0) return;
@@ -486,11 +494,11 @@ int qk_norm_rope_q30(const QkRope& given, cudaStream_t st) {
     p.inv_hd = 1.0 / (double)p.hd;
     const int64_t units = p.M * (p.q.nh + p.k.nh);
     const unsigned grid = (unsigned)((units + QT / 32 - 1) / (QT / 32));
-    if (p.half <= 32) k_qk_q30<1><<<grid, QT, 0, st>>>(p);
-    else if (p.half <= 64) k_qk_q30<2><<<grid, QT, 0, st>>>(p);
-    else if (p.half <= 128) k_qk_q30<4><<<grid, QT, 0, st>>>(p);
-    else if (p.half <= 256) k_qk_q30<8><<<grid, QT, 0, st>>>(p);
-    else k_qk_q30_wide<<<grid, QT, 0, st>>>(p);
+    if (p.half <= 32) launch_early(k_qk_q30<1>, grid, QT, 0, st, 1, p);
+    else if (p.half <= 64) launch_early(k_qk_q30<2>, grid, QT, 0, st, 1, p);
+    else if (p.half <= 128) launch_early(k_qk_q30<4>, grid, QT, 0, st, 1, p);
+    else if (p.half <= 256) launch_early(k_qk_q30<8>, grid, QT, 0, st, 1, p);
+    else launch_early(k_qk_q30_wide, grid, QT, 0, st, 1, p);
     return 1;
 }
 

@@ -287,6 +287,37 @@ def test_streams_and_graphs(ctx):
             assert torch.equal(c.y[:, : c.N], f)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M", [1, 7, 24, 200, 3000])
+def test_calls_that_feed_each_other(ctx, dtype, M):
+    """y = A x, x = B y + x over and over without a pause: each call reads what the one before it wrote and
+    writes what that one read. The same as with a synchronisation after every call."""
+    a, b = Case(ctx, dtype, M, 384, 384, act="gelu_tanh", seed=1), Case(ctx, dtype, M, 384, 384, bias=True, seed=2)
+    start = (a.x * 0.1).to(a.dt)
+
+    def chain(pause):
+        x, y = start.clone(), torch.empty_like(start)
+        torch.cuda.synchronize()
+        for _ in range(25):
+            a.op.apply_device(x.data_ptr(), M, y.data_ptr(), stream=s.cuda_stream)
+            if pause:
+                torch.cuda.synchronize()
+            b.op.apply_device(y.data_ptr(), M, x.data_ptr(), stream=s.cuda_stream)
+            if pause:
+                torch.cuda.synchronize()
+            with torch.cuda.stream(s):
+                x.mul_(0.4)
+        torch.cuda.synchronize()
+        return x, y
+
+    s = torch.cuda.Stream()
+    ref = chain(True)
+    assert bool(ref[0].isfinite().all())
+    for _ in range(3):
+        got = chain(False)
+        assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
 def test_first_call_inside_a_capture():
     """A context whose first calls are captured: nothing they need is made inside the capture."""
     own = slx.Context(0)
