@@ -24,6 +24,15 @@
 //   PAIR  persistent, two CTAs (cta_group::2) on 256 weight rows: each loads its own 128 weight rows and half
 //         of the activation rows, which halves the activation bytes per MMA; the epilogue of a tile runs
 //         under the MMAs of the next (two accumulators).
+// What bounds PAIR is shared memory as much as the tensor pipe: a K block of a 256-column tile takes 512 cycles
+// of MMA and, at 128 bytes a cycle, 250 each for the operands' reads and the TMA's writes plus 170 for the
+// epilogue's staging (K 768): 543 cycles a block measured without a concurrent epilogue, 713 with one. A gated
+// tile has 128 columns an array (two accumulators of it, twice, fill TMEM) and takes 810 where its MMAs take 512.
+// Leaving out the loads of either operand changes the times by 2 to 8 %.
+// Measured (device time, L2 cold inputs; 1654.5 TFLOP/s is the card's measured cuBLAS rate): bf16 8192^3 703 us,
+// 1565 TFLOP/s; 4096 x 4096 x 11008 with bias, GELU and residual 276 us, 1340; 512 x 2048 x 16384 gated 67.5 us,
+// 1018; 8192 x 768 x 2304 27.3 us, 1064; f32 8192 x 768 x 2304 147 us, 197 (1180 of bf16 products); f16
+// 129 x 1001 x 1111 8.0 us. Under the power cap of a long loop the three large ones take 312, 79 and 164 us.
 // Every mbarrier wait is bounded.
 #include <cuda.h>
 
