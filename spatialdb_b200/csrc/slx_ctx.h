@@ -76,9 +76,11 @@ inline int set_err(slx_ctx* c, int code, const char* fmt, ...) {
 #define CK(call)                                                                                 \
     do {                                                                                         \
         cudaError_t e_ = (call);                                                                 \
-        if (e_ != cudaSuccess)                                                                   \
+        if (e_ != cudaSuccess) {                                                                 \
+            cudaGetLastError(); /* reported here: not once more by the next call's check */      \
             return set_err(ctx, e_ == cudaErrorMemoryAllocation ? SLX_EOOM : SLX_ECUDA, "%s: %s", \
                            #call, cudaGetErrorString(e_));                                      \
+        }                                                                                        \
     } while (0)
 
 inline cudaStream_t pick(slx_ctx* ctx, void* s) { return s ? (cudaStream_t)s : ctx->stream; }

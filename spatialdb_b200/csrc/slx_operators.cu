@@ -176,7 +176,8 @@ slx_status slx_linear_prepare(slx_ctx* ctx, int dtype, const uint8_t* d_w, int64
     OnDevice on(ctx->device);
     CK(on.err);
     if (int rc = ensure_pool(ctx)) return rc;
-    std::unique_ptr<slx_linear> h(new slx_linear());
+    std::unique_ptr<slx_linear> h(new (std::nothrow) slx_linear());
+    if (!h) return set_err(ctx, SLX_EOOM, "host memory");
     h->ctx = ctx;
     lin::Plan& p = h->plan;
     p.dtype = dtype; p.N = N; p.K = K; p.act = act; p.gated = d_gate != nullptr;
@@ -328,7 +329,8 @@ slx_status slx_qk_norm_prepare(slx_rope* r, int dtype, int heads, int kv_heads, 
     if (((uintptr_t)d_wq | (uintptr_t)d_wk) % e) return set_err(ctx, SLX_EINVAL, "norm weights not aligned to %d bytes", e);
     OnDevice on(ctx->device);
     CK(on.err);
-    std::unique_ptr<slx_qk_norm> h(new slx_qk_norm());
+    std::unique_ptr<slx_qk_norm> h(new (std::nothrow) slx_qk_norm());
+    if (!h) return set_err(ctx, SLX_EOOM, "host memory");
     h->ctx = ctx;
     h->dtype = dtype; h->heads = heads; h->kv_heads = kv_heads; h->hd = head_dim; h->eps = eps;
     if (int st = copy_vector(ctx, d_wq, (size_t)e * head_dim, &h->wq)) return st;

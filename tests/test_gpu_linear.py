@@ -413,6 +413,17 @@ def test_refusals(ctx):
     c.check()
 
 
+def test_failed_allocation_is_reported_once(ctx):
+    """Weights no device holds: the allocation's failure ends that call alone. (The buffer is not read.)"""
+    w = torch.zeros(64, dtype=torch.float16, device="cuda")
+    n = 1 << 21
+    for dtype, size in ((slx.DTYPE_F32, 2), (slx.DTYPE_F16, 2)):
+        with pytest.raises(slx.SlxError) as e:
+            slx.Linear(dtype, w.data_ptr(), n * n * size, slx.DTYPE_F16, n, n, ctx=ctx)
+        assert e.value.status == slx.SLX_EOOM
+        Case(ctx, "f32", 20, 64, 64).check()
+
+
 def test_handle_outlives_its_context():
     own = slx.Context(0)
     c = Case(own, "bf16", 20, 64, 64)
