@@ -561,6 +561,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     } else if (warp == 1) {
         if (lane == 0 && (MODE != PAIR || rank == 0)) {  // MMA issuer
             const uint32_t idesc = idesc_f16(128 * CG, NT, !p.f16);
+            grid_wait();  // the bounded waits below are for this kernel's copies, not for the kernels ahead
             int use = 0, s = 0;
             uint32_t ph = 0;
             bool ok = true, issued = false;

@@ -370,6 +370,19 @@ def test_wait_that_gives_up_is_reported():
         c.check()
 
 
+def test_wait_limit_counts_from_the_kernels_ahead():
+    """A call queued behind one that runs several times as long as the wait limit: its own waits start when that
+    one has ended. The long call is one weight tile whose sums (promoted every 256 values) wait briefly each."""
+    own = slx.Context(0)
+    long, short = Case(own, "f32", 17, 1 << 19, 128), Case(own, "f32", 40, 512, 256)
+    own.set_option(slx.OPT_WAIT_LIMIT_CYCLES, 400_000)
+    for _ in range(3):
+        long.run()
+        short.run()
+    own.status(slx.STREAM_LEGACY)
+    short.check()
+
+
 def test_empty_and_profile(ctx):
     c = Case(ctx, "bf16", 20, 64, 64)
     c.op.apply_device(0, 0, 0)
