@@ -14,7 +14,7 @@
 // truncates when it adds to an accumulator, which biases long sums, so every 256 values of K both
 // accumulators are added to fp32 registers (rounded to nearest) and started anew.
 //
-// Two forms, the cheaper by an estimate of its cycles (choose):
+// Three forms, the cheapest by an estimate of its cycles (choose):
 //   ONE   one tile at a time. A cluster of S = 1, 2, 4 or 8 CTAs shares the tile, each with a range of the K
 //         blocks, so that few tiles still occupy the SMs. CTA c of S finishes columns c NT / S...: the others
 //         store their partial sums of them into its shared memory, and it adds them in rank order. One
@@ -23,16 +23,20 @@
 //         them (MANUAL), without a pass of its own.
 //   PAIR  persistent, two CTAs (cta_group::2) on 256 weight rows: each loads its own 128 weight rows and half
 //         of the activation rows, which halves the activation bytes per MMA; the epilogue of a tile runs
-//         under the MMAs of the next (two accumulators).
+//         under the MMAs of the next (two accumulators). With a gate a CTA's 128 rows are 64 of the weights and the
+//         same 64 of the gate's, in one accumulator of all 256 columns: they meet in the epilogue's shared memory.
+//   WIDE  (16 bits, gated) pairs with 128 rows of each array a CTA, an accumulator each, on 128 activation rows: for
+//         products of one such tile whose PAIR tiles just miss a wave.
 // What bounds PAIR is shared memory as much as the tensor pipe: a K block of a 256-column tile takes 512 cycles
 // of MMA and, at 128 bytes a cycle, 250 each for the operands' reads and the TMA's writes plus 170 for the
-// epilogue's staging (K 768): 543 cycles a block measured without a concurrent epilogue, 713 with one. A gated
-// tile has 128 columns an array (two accumulators of it, twice, fill TMEM) and takes 810 where its MMAs take 512.
+// epilogue's staging (K 768): 543 cycles a block measured without a concurrent epilogue, 713 with one. Gated, 810
+// (K 2048); with 128 columns of each array in accumulators of their own, the form before, 950.
 // Leaving out the loads of either operand changes the times by 2 to 8 %.
 // Measured (device time, L2 cold inputs; 1654.5 TFLOP/s is the card's measured cuBLAS rate): bf16 8192^3 703 us,
-// 1565 TFLOP/s; 4096 x 4096 x 11008 with bias, GELU and residual 276 us, 1340; 512 x 2048 x 16384 gated 67.5 us,
-// 1018; 8192 x 768 x 2304 27.3 us, 1064; f32 8192 x 768 x 2304 147 us, 197 (1180 of bf16 products); f16
-// 129 x 1001 x 1111 8.0 us. Under the power cap of a long loop the three large ones take 312, 79 and 164 us.
+// 1565 TFLOP/s; 4096 x 4096 x 11008 with bias, GELU and residual 276 us, 1340; 512 x 2048 x 16384 gated 59 us,
+// 1165; 8192 x 768 x 2304 27.3 us, 1064; f32 8192 x 768 x 2304 147 us, 197 (1180 of bf16 products), 512 x
+// 2048 x 8192 gated 169 us, 203 (one array's rows a tile, the form before: 278); f16 129 x 1001 x 1111 8.0 us. Under
+// the power cap of a long loop 4096 x 4096 x 11008 takes 312, the gated product 70 and the f32 one 164 us.
 // Every mbarrier wait is bounded.
 #include <cuda.h>
 
@@ -55,7 +59,7 @@ namespace {
 
 using namespace tc;
 
-enum Mode { ONE = 0, PAIR = 1 };
+enum Mode { ONE = 0, PAIR = 1, WIDE = 2 };
 
 constexpr int EPI = 16;                     // epilogue warps: four groups of one warp per TMEM lane quarter
 constexpr int GROUPS = EPI / 4;
@@ -81,15 +85,16 @@ struct TcParams {
 
 template <int NT, int PLANES, bool GATED, int MODE>
 struct Shape {
-    static constexpr int S = GATED ? 2 : 1;
+    static constexpr bool DUO = MODE != ONE, MIX = GATED && MODE == PAIR;  // a CTA's 128 rows are 64 of the weights and 64 of the gate's
+    static constexpr int S = GATED && !MIX ? 2 : 1;
     static constexpr int ROWB = PLANES == 3 ? 64 : 128;        // bytes of K per operand row and block
     static constexpr int WB = PLANES * TR * ROWB;              // one weight array's block
-    static constexpr int XR = MODE == PAIR ? NT / 2 : NT;      // activation rows this CTA loads
+    static constexpr int XR = DUO ? NT / 2 : NT;      // activation rows this CTA loads
     static constexpr int STAGE = S * WB + PLANES * XR * ROWB;
     static constexpr int ACC = S * (PLANES == 3 ? 2 : 1);      // accumulators of NT columns
     static constexpr int COLS = 2 * ACC * NT;                  // two buffers
     static constexpr int HC = NT / GROUPS;                     // columns of an epilogue group
-    static constexpr int SLAB = HC < 16 || PLANES == 3 || GATED ? 8 : 16;  // columns it moves through shared memory at a time
+    static constexpr int SLAB = HC < 16 || PLANES == 3 || S == 2 ? 8 : 16;  // columns it moves through shared memory at a time
     // the epilogue's shared memory: the groups' staging, or in ONE the partial sums this CTA finishes
     static constexpr int OUT = MODE == ONE ? S * NT * TR * 4 : GROUPS * S * SLAB * TR * 4;
     static constexpr int FIT = (SMEM_MAX - 1024 - 512 - OUT) / STAGE;
@@ -175,12 +180,13 @@ __device__ __forceinline__ uint32_t idesc_f16(int m, int n, int bf16) {
     return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// A thread's share of a tile's outputs: of rows m of y, the values of four weight rows n.. and of four more
-// from n + 64 (a warp's reads of the staged sums then fall on different banks, and its stores are runs of
+// A thread's share of a tile's outputs: of rows m of y, the values of four weight rows n.. and with H = 2 of four
+// more from n + 64 (a warp's reads of the staged sums then fall on different banks, and its stores are runs of
 // 128 bytes or more). FAST: the tile lies inside y and rows take vectors of four values.
-template <class T, bool GATED>
+template <class T, bool GATED, int H>
 struct Columns {
-    float b[8], gb[8];
+    static constexpr int V = 4 * H;
+    float b[V], gb[V];
     int n;
 
     __device__ __forceinline__ void begin(const TcParams& p, int first) {
@@ -189,63 +195,63 @@ struct Columns {
         if (GATED) fill(gb, p.gbias, p.N);
     }
     __device__ __forceinline__ int at(int j) const { return n + (j & 3) + (j >> 2) * 64; }
-    __device__ __forceinline__ void fill(float (&v)[8], const float* from, int N) const {
+    __device__ __forceinline__ void fill(float (&v)[V], const float* from, int N) const {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = from && at(j) < N ? from[at(j)] : 0.0f;
+        for (int j = 0; j < V; j++) v[j] = from && at(j) < N ? from[at(j)] : 0.0f;
     }
 
     struct __align__(4 * sizeof(T)) Four {
         T v[4];
     };
-    struct __align__(16) Residual {
-        Four f[2];
+    struct __align__(8) Residual {
+        Four f[H];
     };
     template <bool FAST>
     __device__ __forceinline__ void load(const TcParams& p, int64_t m, Residual& r) const {
         if (!p.r) return;
         const T* src = (const T*)p.r + m * p.ldr;
         if (FAST) {
-            copy(&r.f[0], src + n);
-            copy(&r.f[1], src + n + 64);
+#pragma unroll
+            for (int h = 0; h < H; h++) copy(&r.f[h], src + n + 64 * h);
         } else if (m < p.M) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
+            for (int j = 0; j < V; j++)
                 if (at(j) < p.N) r.f[j >> 2].v[j & 3] = src[at(j)];
         }
     }
     // Items' sums (and gate sums) to outputs, R rows of m apart `step`.
     template <bool FAST, int R>
-    __device__ __forceinline__ void store(const TcParams& p, int64_t m, int step, float (&v)[8 * R], float (&g)[8 * R],
+    __device__ __forceinline__ void store(const TcParams& p, int64_t m, int step, float (&v)[V * R], float (&g)[V * R],
                                           const Residual (&r)[R]) const {
 #pragma unroll
-        for (int j = 0; j < 8 * R; j++) {
-            v[j] += b[j & 7];
-            if (GATED) g[j] += gb[j & 7];
+        for (int j = 0; j < V * R; j++) {
+            v[j] += b[j % V];
+            if (GATED) g[j] += gb[j % V];
         }
         if (GATED) {
             activate_all<T>(g, p.act);
 #pragma unroll
-            for (int j = 0; j < 8 * R; j++) v[j] *= g[j];
+            for (int j = 0; j < V * R; j++) v[j] *= g[j];
         } else {
             activate_all<T>(v, p.act);
         }
         if (p.r) {
 #pragma unroll
-            for (int j = 0; j < 8 * R; j++) v[j] += to_f(r[j >> 3].f[(j >> 2) & 1].v[j & 3]);
+            for (int j = 0; j < V * R; j++) v[j] += to_f(r[j / V].f[j % V >> 2].v[j & 3]);
         }
 #pragma unroll
         for (int i = 0; i < R; i++) {
             const int64_t row = m + i * step;
             T* dst = (T*)p.y + row * p.ldo;
-            Four o[2];
+            Four o[H];
 #pragma unroll
-            for (int j = 0; j < 8; j++) o[j >> 2].v[j & 3] = from_f<T>(v[8 * i + j]);
+            for (int j = 0; j < V; j++) o[j >> 2].v[j & 3] = from_f<T>(v[V * i + j]);
             if (FAST) {
-                copy(dst + n, &o[0]);
-                copy(dst + n + 64, &o[1]);
+#pragma unroll
+                for (int h = 0; h < H; h++) copy(dst + n + 64 * h, &o[h]);
             } else if (row < p.M) {
 #pragma unroll
-                for (int j = 0; j < 8; j++)
+                for (int j = 0; j < V; j++)
                     if (at(j) < p.N) dst[at(j)] = o[j >> 2].v[j & 3];
             }
         }
@@ -449,7 +455,8 @@ __global__ void __launch_bounds__(LT, 1)
 k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmg,
             const __grid_constant__ TcParams p) {
     using Sh = Shape<NT, PLANES, GATED, MODE>;
-    constexpr int S = Sh::S, ST = Sh::STAGES, ROWB = Sh::ROWB, CG = MODE == PAIR ? 2 : 1;
+    constexpr int S = Sh::S, ST = Sh::STAGES, ROWB = Sh::ROWB, CG = Sh::DUO ? 2 : 1;
+    constexpr bool DUO = Sh::DUO, MIX = Sh::MIX;
     extern __shared__ uint8_t smem_raw[];
     // The pair's MMA reads both CTAs' operands at the same offsets: the dynamic area starts at the same
     // address in every CTA of a launch, so its rounded-up base does too.
@@ -490,7 +497,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     }
     fence_before();
     __syncthreads();
-    if (MODE == PAIR) cluster_sync();   // both CTAs' barriers exist before either is signalled
+    if (DUO) cluster_sync();   // both CTAs' barriers exist before either is signalled
     if (MODE == ONE) cluster_arrive();  // waited for before the first store to another CTA
     bool met = false;
     fence_after();
@@ -498,7 +505,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
 
     // This CTA's tiles and K blocks.
     const int rank = (int)cluster_rank(), split = 1 << p.log2_split;
-    const int tiles_n = MODE == PAIR ? (p.tiles_n + 1) / 2 : p.tiles_n;
+    const int tiles_n = DUO && !MIX ? (p.tiles_n + 1) / 2 : p.tiles_n;
     const int tile0 = MODE == ONE ? (int)blockIdx.x >> p.log2_split : (int)blockIdx.x / CG;
     const int tstep = MODE == ONE ? p.tiles : (int)gridDim.x / CG;
     const int kb0 = MODE == ONE ? (int)(((int64_t)p.nkb * rank) >> p.log2_split) : 0;
@@ -509,12 +516,21 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
         if (lane == 0) {  // producer, running ahead across tiles
             auto load_w = [&](int kb, int stage, int64_t blk0) {
                 const uint32_t dst = sbase + stage * Sh::STAGE, bar = full0 + 8 * stage;
-                if (MODE == PAIR) {
+                if (DUO) {
                     const uint32_t lead = peer_addr(bar, 0);
                     if (rank == 0) mbar_expect_tx(bar, 2 * Sh::STAGE);
                     const int line = (int)((blk0 + kb) * (Sh::WB / 128));
-                    pair_load_2d(dst, &tmw, 0, line, lead);
-                    if (GATED) pair_load_2d(dst + Sh::WB, &tmg, 0, line, lead);
+                    if (MIX) {  // of every part's block this CTA's half of the weights' rows, then of the gate's
+                        constexpr int HALF = TR * ROWB / 2;
+#pragma unroll
+                        for (int q = 0; q < PLANES; q++) {
+                            pair_load_2d(dst + 2 * q * HALF, &tmw, 0, line + (2 * q + rank) * (HALF / 128), lead);
+                            pair_load_2d(dst + 2 * q * HALF + HALF, &tmg, 0, line + (2 * q + rank) * (HALF / 128), lead);
+                        }
+                    } else {
+                        pair_load_2d(dst, &tmw, 0, line, lead);
+                        if (GATED) pair_load_2d(dst + Sh::WB, &tmg, 0, line, lead);
+                    }
                 } else {
                     mbar_expect_tx(bar, MANUAL ? S * Sh::WB : Sh::STAGE);
                     bulk_load(dst, p.w + (blk0 + kb) * Sh::WB, Sh::WB, bar);
@@ -527,8 +543,8 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
             for (int t = tile0; ok && t < p.tiles; t += tstep) {
                 int tm, tn;
                 tile_at(p, tiles_n, t, tm, tn);
-                const int m0 = tm * NT + (MODE == PAIR ? rank * Sh::XR : 0);
-                const int64_t blk0 = (int64_t)(MODE == PAIR ? 2 * tn + rank : tn) * p.nkb;
+                const int m0 = tm * NT + (DUO ? rank * Sh::XR : 0);
+                const int64_t blk0 = (int64_t)(DUO && !MIX ? 2 * tn + rank : tn) * p.nkb;
                 // Weights are the handle's own memory, which no kernel in the stream writes: the first stages' are
                 // asked for before the kernels ahead of this one are waited for, the activations after it.
                 const int ahead = MODE == ONE ? (kb1 - kb0 < ST ? kb1 - kb0 : ST) : 0;
@@ -543,13 +559,13 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                     }
                     if (!asked) load_w(kb, s, blk0);
                     const uint32_t dst = sbase + s * Sh::STAGE + S * Sh::WB, bar = full0 + 8 * s;
-                    if (MODE == PAIR) pair_load_3d(dst, &tmx, kb * (ROWB / 2), m0, 0, peer_addr(bar, 0));
+                    if (DUO) pair_load_3d(dst, &tmx, kb * (ROWB / 2), m0, 0, peer_addr(bar, 0));
                     else if (!MANUAL) tma_load_3d(dst, &tmx, kb * (ROWB / 2), m0, 0, bar);
                     if (++s == ST) { s = 0; ph ^= 1u; }
                 }
             }
             if (!ok) {  // let copies still in flight land before the CTA exits (they always complete)
-                if (MODE != PAIR && !MANUAL) {
+                if (!DUO && !MANUAL) {
                     for (int j = done - ST < 0 ? 0 : done - ST; j < done; j++)
                         mbar_wait(full0 + 8 * (j % ST), (uint32_t)(j / ST) & 1u);
                 } else {  // their barriers also count the other CTA's copies, or rows that may not come: a millisecond
@@ -559,7 +575,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && (MODE != PAIR || rank == 0)) {  // MMA issuer
+        if (lane == 0 && (!DUO || rank == 0)) {  // MMA issuer
             const uint32_t idesc = idesc_f16(128 * CG, NT, !p.f16);
             grid_wait();  // the bounded waits below are for this kernel's copies, not for the kernels ahead
             int use = 0, s = 0;
@@ -618,17 +634,18 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
         const int q4 = warp & 3, part = (warp - 2) >> 2, row = 32 * q4 + lane;
         constexpr int HC = Sh::HC, SLAB = Sh::SLAB;
         const uint32_t tbase = tmem + ((uint32_t)(32 * q4) << 16) + part * HC;
-        const uint32_t free0 = MODE == PAIR ? peer_addr(tfree0, 0) : tfree0;
+        const uint32_t free0 = DUO ? peer_addr(tfree0, 0) : tfree0;
         float* st = out_stage + part * S * SLAB * TR;
         const int tid = (int)threadIdx.x - 64 - 128 * part, col = tid >> 4;
         const float* src = st + col * TR + (tid & 15) * 4;
+        constexpr int OH = MIX ? 1 : 2;  // runs of four outputs a thread has in a row of y
         grid_wait();  // x, the residual and y belong to the kernels ahead until they have ended
         int use = 0;
         auto release = [&](int buf) {  // this warp has read the buffer
             fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (MODE == PAIR) peer_arrive(free0 + 8 * buf);
+                if (DUO) peer_arrive(free0 + 8 * buf);
                 else mbar_arrive(tfree0 + 8 * buf);
             }
         };
@@ -636,8 +653,8 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
             int tm, tn;
             tile_at(p, tiles_n, t, tm, tn);
             const int64_t m0 = (int64_t)tm * NT + part * HC;
-            const int n0 = (MODE == PAIR ? 2 * tn + rank : tn) * TR;
-            Columns<T, GATED> out;
+            const int n0 = MIX ? tn * TR + rank * (TR / 2) : (DUO ? 2 * tn + rank : tn) * TR;
+            Columns<T, GATED, OH> out;
             out.begin(p, n0 + (tid & 15) * 4);
             // The rows of two accumulator chunks ahead of the one being read: the MMAs of chunk i wait for the
             // sums of chunk i - 2 to be read, so rows past chunk i + 1 must not be waited for before that.
@@ -704,7 +721,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                 auto slab = [&](int c, auto fast) {
                     constexpr bool FAST = decltype(fast)::value;
                     constexpr int R = SLAB / 8;
-                    typename Columns<T, GATED>::Residual res[R];
+                    typename Columns<T, GATED, OH>::Residual res[R];
 #pragma unroll
                     for (int i = 0; i < R; i++) out.template load<FAST>(p, m0 + c + 8 * i + col, res[i]);
 #pragma unroll
@@ -717,16 +734,17 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                     }
                     if (PLANES == 1 && c + SLAB == HC) release(buf);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                    alignas(16) float v[8 * R], g[8 * R];
+                    alignas(16) float v[4 * OH * R], g[4 * OH * R];
 #pragma unroll
                     for (int i = 0; i < 2 * R; i++) {
-                        *(float4*)(v + 4 * i) = *(const float4*)(src + (i >> 1) * 8 * TR + (i & 1) * 64);
-                        if (GATED) *(float4*)(g + 4 * i) = *(const float4*)(src + (SLAB + (i >> 1) * 8) * TR + (i & 1) * 64);
+                        float* to = MIX && (i & 1) ? g + 4 * (i >> 1) : v + 4 * (MIX ? i >> 1 : i);
+                        *(float4*)to = *(const float4*)(src + (i >> 1) * 8 * TR + (i & 1) * 64);
+                        if (S == 2) *(float4*)(g + 4 * i) = *(const float4*)(src + (SLAB + (i >> 1) * 8) * TR + (i & 1) * 64);
                     }
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
                     out.template store<FAST, R>(p, m0 + c + col, 8, v, g, res);
                 };
-                if (p.vec && n0 + TR <= p.N && m0 + HC <= p.M) {
+                if (p.vec && n0 + 64 * OH <= p.N && m0 + HC <= p.M) {
                     if (PLANES == 1) {
 #pragma unroll 1
                         for (int c = 0; c < HC; c += SLAB) slab(c, std::true_type{});
@@ -747,8 +765,8 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     fence_before();
     __syncwarp();
     if (MODE == ONE && !met) cluster_wait();
-    Columns<T, GATED> last;
-    typename Columns<T, GATED>::Residual res[1];
+    Columns<T, GATED, 2> last;
+    typename Columns<T, GATED, 2>::Residual res[1];
     const int chunk = (int)threadIdx.x & 15, first = ((int)threadIdx.x - 64) >> 4;
     int tm = 0, tn = 0;
     int64_t mr = 0;
@@ -897,14 +915,15 @@ bool launch(const Plan& pl, const Call& c, const Operands& op, int log2_split, c
     } else if (!tc::encode_rows_planes(&tmx, op.x, op.width, c.M, op.ldx, PLANES, pl.bk(), Sh::XR)) {
         return false;
     }
-    if (MODE == PAIR) {  // the weights' blocks as lines of 128 bytes, swizzled already
+    if (Sh::DUO) {  // the weights' blocks as lines of 128 bytes, swizzled already
         const int64_t lines = pl.tile_bytes() / 128;
-        if (!tc::encode_rows_u16(&tmw, pl.tiles, 64, lines, 64, Sh::WB / 128)) return false;
-        if (GATED && !tc::encode_rows_u16(&tmg, pl.gtiles, 64, lines, 64, Sh::WB / 128)) return false;
+        const int box = Sh::MIX ? TR * Sh::ROWB / 2 / 128 : Sh::WB / 128;
+        if (!tc::encode_rows_u16(&tmw, pl.tiles, 64, lines, 64, box)) return false;
+        if (GATED && !tc::encode_rows_u16(&tmg, pl.gtiles, 64, lines, 64, box)) return false;
     } else {
         tmw = tmx;
     }
-    if (!GATED || MODE != PAIR) tmg = tmw;
+    if (!GATED || !Sh::DUO) tmg = tmw;
     TcParams p;
     p.w = pl.tiles; p.g = pl.gtiles; p.bias = pl.bias; p.gbias = pl.gbias;
     p.r = c.r; p.y = c.y; p.ldr = c.ldr; p.ldo = c.ldo;
@@ -914,19 +933,19 @@ bool launch(const Plan& pl, const Call& c, const Operands& op, int log2_split, c
     p.vec = fours(c.y, c.ldo) && (!c.r || fours(c.r, c.ldr));
     p.tiles_n = pl.tiles_n();
     p.tiles_m = (int)((c.M + NT - 1) / NT);
-    p.tiles = p.tiles_m * (MODE == PAIR ? (p.tiles_n + 1) / 2 : p.tiles_n);
+    p.tiles = p.tiles_m * (Sh::DUO && !Sh::MIX ? (p.tiles_n + 1) / 2 : p.tiles_n);
     p.log2_split = log2_split;
     p.err = c.err;
     p.wait_limit = c.wait_limit > 0 ? c.wait_limit : tc::kWaitCycles;
     p.stall_mma = c.stall_mma;
     int grid = p.tiles << log2_split;
-    if (MODE == PAIR) {
+    if (Sh::DUO) {
         static std::atomic<int> clusters{0};
         int n = clusters.load();
         if (!n) clusters.store(n = resident_clusters((const void*)fn, Sh::SMEM, 2));
         grid = 2 * std::min(p.tiles, n);
     }
-    const int size = MODE == PAIR ? 2 : 1 << log2_split;
+    const int size = Sh::DUO ? 2 : 1 << log2_split;
     return launch_early(fn, dim3((unsigned)grid), dim3(LT), Sh::SMEM, st, size, tmx, tmw, tmg, p) == cudaSuccess;
 }
 
@@ -942,14 +961,16 @@ bool run_one(const Plan& pl, const Call& c, const Operands& op, const Choice& ch
 }
 template <class T, int PLANES, bool GATED>
 bool run_pair(const Plan& pl, const Call& c, const Operands& op, const Choice& ch, cudaStream_t st) {
-    constexpr int W = (PLANES == 3 ? 128 : 256) / (GATED ? 2 : 1);
+    constexpr int W = PLANES == 3 ? 128 : 256;
     if (ch.nt == W) return launch<T, W, PLANES, GATED, PAIR, false>(pl, c, op, 0, st);
     if (ch.nt == W / 2) return launch<T, W / 2, PLANES, GATED, PAIR, false>(pl, c, op, 0, st);
-    return launch<T, W / 4 < 32 ? 32 : W / 4, PLANES, GATED, PAIR, false>(pl, c, op, 0, st);
+    return launch<T, W / 4, PLANES, GATED, PAIR, false>(pl, c, op, 0, st);
 }
 template <class T, int PLANES, bool GATED>
 bool run(const Plan& pl, const Call& c, const Operands& op, const Choice& ch, cudaStream_t st) {
     if (ch.mode == PAIR) return run_pair<T, PLANES, GATED>(pl, c, op, ch, st);
+    if constexpr (GATED && PLANES == 1)
+        if (ch.mode == WIDE) return launch<T, 128, PLANES, GATED, WIDE, false>(pl, c, op, 0, st);
     if constexpr (PLANES == 3) return run_one<T, PLANES, GATED, true>(pl, c, op, ch, st);
     else return tma_rows(pl, c) ? run_one<T, PLANES, GATED, false>(pl, c, op, ch, st) : run_one<T, PLANES, GATED, true>(pl, c, op, ch, st);
 }
@@ -973,16 +994,24 @@ void layout(const Plan& p, const void* w, uint8_t* tiles, float* rows, cudaStrea
 }
 
 // The form and tile of a call, by an estimate of its SM cycles. Fixed parts and rates as measured
-// (clock64 stamps in the kernel, and every form and tile of 40 shapes timed): about 3000 cycles from launch to the first MMA, a K block the larger
-// of its MMAs (64 cycles each up to N = 128, N / 2 above) and its bytes at 56 a cycle, 1500 cycles for the
-// exchange in a cluster and 64 bytes a cycle stored in it, four outputs a cycle in the epilogue. Clusters of
-// 8 and 4 fit 15 and 33 times, pairs on all SMs.
+// (clock64 stamps in the kernel, and every form and tile of 60 shapes timed): about 3000 cycles from launch to the
+// first MMA, a K block the larger of its MMAs (64 cycles each up to N = 128, N / 2 above) and its bytes at 56 a
+// cycle, 1500 cycles for the exchange in a cluster and 64 bytes a cycle stored in it, four outputs a cycle in the
+// epilogue. Clusters of 8 and 4 fit 15 and 33 times, pairs on all SMs. Gated 16-bit blocks wait for their bytes:
+// 3300 cycles of latency over the stages in ONE, 420 cycles and their bytes at 100 a cycle in PAIR, 1000 in WIDE.
+// 128 x 4096 x 11008, 86 tiles of 128 rows on 74 pairs: WIDE 41 us, PAIR 49, ONE 57; 512 x 2048 x 16384: PAIR 60,
+// WIDE 68, ONE 120.
 Choice choose(const Plan& p, const Call& c) {
     const int64_t M = c.M;
-    const bool pass = !tma_rows(p, c);  // PAIR needs the rows split or packed, ONE loads them itself
+    const bool pass = !tma_rows(p, c);  // pairs need the rows split or packed, ONE loads them itself
     const int S = p.gated ? 2 : 1, planes = p.planes(), rowb = planes == 3 ? 64 : 128;
     const int steps = planes == 3 ? 12 : 4, sms = device_sm_count();
-    const int widest = planes == 3 ? 128 / S : 256 / S;  // accumulators in TMEM
+    const int widest = planes == 3 ? 128 / S : 256 / S, pair_widest = planes == 3 ? 128 : 256;  // accumulators in TMEM
+    // Cycles of a K block whose weights come from memory (3300 bytes a cycle), read by `ctas` CTAs at a time; those of
+    // up to GROUP_M activation tiles share three quarters of them.
+    auto dram = [](double ctas, double bytes, double tiles_m) {
+        return ctas * bytes / 3300.0 / (0.25 + 0.75 * std::min<double>(tiles_m, GROUP_M));
+    };
     Choice best;
     for (int nt = 32; nt <= 256; nt *= 2) {
         const double tiles_m = (double)((M + nt - 1) / nt), mma = std::max(64, nt / 2);
@@ -995,19 +1024,27 @@ Choice choose(const Plan& p, const Call& c) {
                 const double tiles = tiles_m * p.tiles_n();
                 const double waves = std::ceil(tiles / fit);
                 double block = std::max(S * steps * mma, (S * planes * TR * rowb + planes * nt * rowb) / 56.0);
+                if (p.gated && planes == 1) {
+                    const int stage = (2 * TR + nt) * rowb, stages = std::min(8, (SMEM_MAX - 1536 - 2 * nt * TR * 4) / stage);
+                    block = std::max({block, 3300.0 / stages, dram(std::min<double>(tiles * split, sms), 2 * TR * rowb, tiles_m)});
+                }
                 if (pass) block = std::max(block, planes == 3 ? 1100.0 + 6.0 * nt : 200.0 + 22.0 * nt);
                 const double t = waves * (3000 + std::ceil((double)p.nkb() / split) * block + out / split +
                                           (l ? 1500 + S * rows * TR * 4 / 64.0 : rows * TR * S * 4 / 256.0));
                 if (!best.nt || t < best.cycles) best = Choice{nt, ONE, l, t};
             }
         }
-        if (nt <= widest && nt * 4 >= widest) {
-            const double tiles = tiles_m * ((p.tiles_n() + 1) / 2);
-            const double block = std::max(S * steps * mma * 1.15, (S * planes * TR * rowb + planes * nt / 2 * rowb) / 56.0);
+        for (const int mode : {PAIR, WIDE}) {
+            if (mode == PAIR ? nt > pair_widest || nt * 4 < pair_widest : !p.gated || planes == 3 || nt != 128) continue;
+            const bool mix = p.gated && mode == PAIR;
+            const double tiles = tiles_m * (mix ? p.tiles_n() : (p.tiles_n() + 1) / 2), sums = rows * TR * (mode == WIDE ? 2 : 1) / 4.0;
+            const double loads = planes * rowb * (TR + nt / 2);
+            double block = mode == WIDE ? 1000.0 : mix && planes == 1 ? 420.0 + loads / 100.0 : std::max(steps * mma * 1.15, loads / 56.0);
+            if (mix && planes == 1) block = std::max(block, dram(std::min<double>(2 * tiles, sms), TR * rowb, tiles_m));
             const double work = p.nkb() * block;
-            double t = 4500 + std::ceil(tiles / (sms / 2)) * std::max(work, out) + std::min(work, out);
+            double t = 4500 + std::ceil(tiles / (sms / 2)) * std::max(work, sums) + std::min(work, sums);
             if (pass) t += 3500 + (double)M * p.K * (planes == 3 ? 10 : 4) / 3000.0;
-            if (t < best.cycles) best = Choice{nt, PAIR, 0, t};
+            if (t < best.cycles) best = Choice{nt, mode, 0, t};
         }
     }
     return best;
@@ -1022,7 +1059,7 @@ int tc(const Plan& p, const Call& c, const Choice& ch, void* ws, cudaStream_t st
     const bool direct = tma_rows(p, c);
     Operands op{c.x, c.ldx, p.K};
     int n = 0;
-    if (!direct && ch.mode == PAIR) {
+    if (!direct && ch.mode != ONE) {
         const int kp = kp_of(p);
         const unsigned grid = grid_for(c.M * (kp / 8));
         if (p.planes() == 3) k_split_x<<<grid, 256, 0, st>>>((const float*)c.x, c.ldx, c.M, p.K, kp, (uint16_t*)ws);

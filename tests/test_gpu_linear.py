@@ -135,6 +135,15 @@ def test_gated(ctx, dtype, M, K, N):
     Case(ctx, dtype, M, K, N, act="gelu_tanh", gated=True, bias=True, residual=True, pad=8).check()
 
 
+@pytest.mark.parametrize("dtype,M,K,N,pad", [("bf16", 120, 1024, 9900, 0), ("f16", 128, 2048, 11008, 0), ("bf16", 77, 1111, 10001, 1),
+                                             ("f16", 513, 640, 2050, 1), ("bf16", 600, 768, 2048, 0), ("bf16", 130, 512, 9600, 0),
+                                             ("f16", 300, 200, 70, 0), ("f32", 512, 1024, 2050, 0), ("f32", 700, 333, 1300, 1)])
+def test_gated_pairs(ctx, dtype, M, K, N, pad):
+    """Gated products on pairs of CTAs: half of each array's rows a CTA, and whole blocks of both for one activation tile."""
+    Case(ctx, dtype, M, K, N, act="silu", gated=True, bias=True, residual=True, pad=pad).check()
+    Case(ctx, dtype, M, K, N, act="gelu_tanh", gated=True, pad=pad, seed=1).check()
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("M", [2, 70])
