@@ -364,9 +364,11 @@ def test_wait_that_gives_up_is_reported():
     """The tensor-core kernel's bounded waits: with its MMA warp idle and a short limit the call ends,
     the status is reported once, and the context computes the next call."""
     own = slx.Context(0)
-    # one tile a cluster (rows by TMA, by the epilogue's warps) and pairs
-    for dtype, M, N in (("bf16", 40, 128), ("f32", 40, 256), ("f32", 3000, 2000), ("bf16", 2000, 3000)):
-        c = Case(own, dtype, M, 512, N)
+    # one tile a cluster (rows by TMA, by the epilogue's warps) and pairs, gated with both arrays' rows in a tile and wide
+    for dtype, M, K, N, gated in (("bf16", 40, 512, 128, False), ("f32", 40, 512, 256, False), ("f32", 3000, 512, 2000, False),
+                                  ("bf16", 2000, 512, 3000, False), ("f16", 513, 512, 4096, True), ("f32", 513, 512, 4096, True),
+                                  ("bf16", 128, 1024, 11008, True)):
+        c = Case(own, dtype, M, K, N, act="silu" if gated else "none", gated=gated)
         own.set_option(slx.OPT_WAIT_LIMIT_CYCLES, 2_000_000)
         own.set_option(slx.OPT_TEST_STALL_MMA, 1)
         c.run()
