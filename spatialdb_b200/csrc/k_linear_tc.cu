@@ -102,6 +102,7 @@ struct Shape {
     static constexpr int GROUPS_X = XR * (ROWB / 16) / 32;     // MANUAL: groups of 32 chunks of eight values a block
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + OUT + 1024 + 512;
     static_assert(COLS <= 512 && STAGES >= 2, "tile does not fit");
+    static_assert(2 * SMEM > SMEM_MAX, "two CTAs on an SM would share its tensor memory");
 };
 
 template <int CG>
@@ -469,7 +470,6 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     uint32_t* tmem_slot = (uint32_t*)(bars + 2 * ST + 5);
     __shared__ int s_fail;
 
-    grid_release();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long limit = p.wait_limit;
     if (threadIdx.x == 0) {
@@ -497,6 +497,9 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
     }
     fence_before();
     __syncthreads();
+    // Not before this CTA holds its tensor memory: a kernel let in earlier, of another library perhaps, could take the
+    // columns first and hold them while it waits for this kernel, which would then wait for them without a limit.
+    grid_release();
     if (DUO) cluster_sync();   // both CTAs' barriers exist before either is signalled
     if (MODE == ONE) cluster_arrive();  // waited for before the first store to another CTA
     bool met = false;
