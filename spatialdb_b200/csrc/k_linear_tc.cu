@@ -8,11 +8,13 @@
 // epilogue: 16 columns at a time go from TMEM through shared memory, so that bias, activation, gate,
 // residual and the one rounding run on runs of a row's outputs with vector accesses.
 //
-// f32 (PLANES = 3): each value is the exact sum of three bf16 parts (8 significant bits each, by
-// truncation), x = x1 + x2 + x3. x1 w1 goes to one accumulator, the corrections x1 w2 + x2 w1 + x2 w2 +
-// x1 w3 + x3 w1 (at most 2^-8 of it) to another; what is left out is below 2^-23 |x| |w|. The tensor core
-// truncates when it adds to an accumulator, which biases long sums, so every 256 values of K both
-// accumulators are added to fp32 registers (rounded to nearest) and started anew.
+// f32 (PLANES = 3): each value is the exact sum of three bf16 parts, each rounded to nearest, x = x1 + x2 + x3 with
+// |x2| <= 2^-8 |x| and |x3| <= 2^-17 |x|. x1 w1 goes to one accumulator, the corrections x1 w2 + x2 w1 + x2 w2 +
+// x1 w3 + x3 w1 (at most 2^-6.9 of it) to another; x2 w3 + x3 w2 + x3 w3, left out, is at most 2^-23.9 |x| |w| and of
+// either sign. (Parts cut off instead of rounded leave out up to 2^-21 |x| |w|, all of the product's sign: 7.8 x 2^-24 of
+// 1.0078^2.) The tensor core truncates when it adds to an accumulator, which biases long sums, so every 256 values
+// of K both accumulators are added to fp32 registers (rounded to nearest) and started anew. x1 w1 may pass the sum it
+// stands for by 2^-7 of it: a sum within 2^-7 of the largest finite value may end infinite.
 //
 // Three forms, the cheapest by an estimate of its cycles (choose):
 //   ONE   one tile at a time. A cluster of S = 1, 2, 4 or 8 CTAs shares the tile, each with a range of the K
@@ -285,32 +287,41 @@ __device__ __forceinline__ void tile_at(const TcParams& p, int tiles_n, int t, i
     tn = i / width;
 }
 
-// The three bf16 parts of eight fp32 values, each the leading eight significant bits of what is left (cut
-// off, so no part overflows): their sum is the value exactly. Of a value that is not finite the first part
-// keeps it (a NaN stays one) and the others are zero.
+// The three bf16 parts of eight fp32 values, each what is left rounded to nearest: x1 takes 8 of the 24 significant
+// bits, what it leaves is a multiple of x's last place and at most 2^-8 of x, what x2 leaves of that at most 2^-17,
+// which fits x3: the sum is the value exactly, and the parts' signs favour no side. A finite value whose x1 would
+// round to infinity has its x1 cut off instead. Of a value that is not finite the first part keeps it (a NaN stays
+// one) and the others are zero.
 __device__ __forceinline__ void split3(const float (&f)[8], uint4 (&part)[3]) {
     float r[8], q[8];
     uint32_t w[3][4];
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        r[j] = f[j] - __uint_as_float(__float_as_uint(f[j]) & 0xFFFF0000u);
-        q[j] = r[j] - __uint_as_float(__float_as_uint(r[j]) & 0xFFFF0000u);
-    }
+    auto high = [](float v) { return __float_as_uint(v) & 0xFFFF0000u; };
+    auto pair = [](float lo, float hi) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *(const uint32_t*)&h;
+    };
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        w[0][j] = __byte_perm(__float_as_uint(f[2 * j]), __float_as_uint(f[2 * j + 1]), 0x7632);
-        w[1][j] = __byte_perm(__float_as_uint(r[2 * j]), __float_as_uint(r[2 * j + 1]), 0x7632);
-        w[2][j] = __byte_perm(__float_as_uint(q[2 * j]), __float_as_uint(q[2 * j + 1]), 0x7632);
+        const int a = 2 * j, b = a + 1;
+        w[0][j] = pair(f[a], f[b]);
+        r[a] = f[a] - __uint_as_float(w[0][j] << 16);
+        r[b] = f[b] - __uint_as_float(high(__uint_as_float(w[0][j])));
+        w[1][j] = pair(r[a], r[b]);
+        q[a] = r[a] - __uint_as_float(w[1][j] << 16);
+        q[b] = r[b] - __uint_as_float(high(__uint_as_float(w[1][j])));
+        w[2][j] = pair(q[a], q[b]);
     }
     const float sum = ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
-    if (isnan(sum)) {  // inf - inf and NaN - NaN: some value is not finite
+    if (!isfinite(sum)) {  // some value, or its first part, is not finite (finite remainders cannot reach the largest value)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            if (isfinite(f[j])) continue;
-            const uint32_t keep = j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-            if (isnan(f[j])) w[0][j / 2] |= 0x00400040u & ~keep;
-            w[1][j / 2] &= keep;
-            w[2][j / 2] &= keep;
+            if (isfinite(r[j])) continue;
+            const float x1 = __uint_as_float(high(f[j])), x2 = f[j] - x1;
+            const bool cut = isfinite(f[j]);
+            const float c2 = __bfloat162float(__float2bfloat16_rn(x2));
+            const uint32_t p[3] = {high(f[j]) | (isnan(f[j]) ? 0x00400000u : 0u), cut ? high(c2) : 0u, cut ? high(x2 - c2) : 0u};
+#pragma unroll
+            for (int i = 0; i < 3; i++) w[i][j / 2] = j & 1 ? (w[i][j / 2] & 0x0000FFFFu) | p[i] : (w[i][j / 2] & 0xFFFF0000u) | p[i] >> 16;
         }
     }
 #pragma unroll

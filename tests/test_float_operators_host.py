@@ -1,6 +1,9 @@
 """Host-side checks of the float operators' sources and helpers that need no device."""
+import math
 import os
 import re
+
+import numpy as np
 
 from spatialdb_b200 import build
 
@@ -20,3 +23,39 @@ def test_dependents_start_after_the_tensor_memory_is_taken():
     assert len(alloc) == 2 and len(release) == 1
     barrier = body.index("__syncthreads()", max(alloc))
     assert max(alloc) < barrier < release[0] < body.index("grid_wait()")
+
+
+def nearest(v):
+    """fp32 values rounded to the nearest bf16 (ties to even), finite where cutting off would be."""
+    u = v.view(np.uint32)
+    up = ((u + np.uint32(0x7FFF) + ((u >> np.uint32(16)) & np.uint32(1))) & np.uint32(0xFFFF0000)).view(np.float32)
+    return np.where(np.isfinite(up), up, (u & np.uint32(0xFFFF0000)).view(np.float32))
+
+
+def test_rounded_bf16_parts_sum_to_the_value():
+    """x = x1 + x2 + x3 exactly, with remainders of 2^-8 and 2^-17 (twice that where x1 is cut off at the range's top),
+    the product of two such sums short of six of its nine terms by 2^-23.9, and no bias to one side."""
+    rng = np.random.default_rng(6)
+    near = (1 + rng.integers(0, 1 << 23, 20000) * 2.0 ** -23) * 2.0 ** rng.integers(-90, 120, 20000)
+    ties = (1 + (2 * rng.integers(0, 128, 2000) + 1) * 2.0 ** -8 + rng.integers(-2, 3, 2000) * 2.0 ** -23) * 2.0 ** rng.integers(-90, 120, 2000)
+    v = np.concatenate([near, ties, -near, [0.0, -0.0, 1.0, 1 + 2 ** -23, 2 - 2 ** -23]]).astype(np.float32)
+    top = np.array([3.4028234e38, -3.4028234e38, 3.3961775e38, 3.39e38, 3.395e38], np.float32)
+    for values, first in ((v, 2.0 ** -8), (top, 2.0 ** -7)):
+        a = nearest(values)
+        r = values - a
+        b = nearest(r)
+        c = nearest(r - b)
+        assert (a.astype(np.float64) + b + c == values).all() and np.isfinite(a).all()
+        size = np.abs(values.astype(np.float64))
+        assert (np.abs(b) <= first * size).all() and (np.abs(c) <= first * 2.0 ** -9 * size).all()
+    x, w = rng.permutation(np.abs(near)).astype(np.float32), np.abs(near).astype(np.float32)
+
+    def parts(v):
+        a = nearest(v)
+        b = nearest(v - a)
+        return [t.astype(np.float64) for t in (a, b, v - a - b)]
+
+    (_, x2, x3), (_, w2, w3) = parts(x), parts(w)
+    left = (x2 * w3 + x3 * w2 + x3 * w3) / (x.astype(np.float64) * w)
+    assert np.abs(left).max() <= 2.0 ** -23.9
+    assert abs(left.mean()) <= 6 * left.std() / math.sqrt(left.size)

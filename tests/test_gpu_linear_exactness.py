@@ -1,0 +1,70 @@
+"""What the float linear operator's results hold at the ends of their range, against the formula in 64 bits: the
+three-part split of f32 products, infinities in them, the activations' tails. Each tolerance is relative to the
+output and derived beside its test."""
+import math
+
+import pytest
+
+import spatialdb_b200 as slx
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+TYPES = {"f32": (slx.DTYPE_F32, torch.float32), "f16": (slx.DTYPE_F16, torch.float16), "bf16": (slx.DTYPE_BF16, torch.bfloat16)}
+ACTS = {"silu": slx.ACT_SILU, "gelu_tanh": slx.ACT_GELU_TANH, "gelu_erf": slx.ACT_GELU_ERF}
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return slx.Context(0)
+
+
+def linear(ctx, x, w, dtype, act=0, gate=None):
+    """act(x . w^T), or with gate weights act(x . gate^T) * (x . w^T)."""
+    code, dt = TYPES[dtype]
+    size = w.numel() * w.element_size()
+    torch.cuda.synchronize()
+    op = slx.Linear(code, w.data_ptr(), size, code, *w.shape, act=act, d_gate=gate.data_ptr() if gate is not None else 0,
+                    gate_bytes=size if gate is not None else 0, ctx=ctx)
+    y = torch.full((x.shape[0], w.shape[0]), 7.0, dtype=dt, device="cuda")
+    op.apply_device(x.data_ptr(), x.shape[0], y.data_ptr(), ldx=x.stride(0), stream=slx.STREAM_LEGACY)
+    ctx.status(slx.STREAM_LEGACY)
+    return y
+
+
+# ---- f32 products from three bf16 parts ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("value", [1 + 2.0 ** -7 - 2.0 ** -23, 1 + 2.0 ** -8 - 2.0 ** -23, 1 + 2.0 ** -8 + 2.0 ** -16, 1.9999999,
+                                   1 + 2.0 ** -9 + 2.0 ** -17])
+@pytest.mark.parametrize("M", [40, 600])
+@pytest.mark.parametrize("K", [1, 16, 32, 256, 768, 4096])
+def test_f32_products_of_one_sign(ctx, M, K, value):
+    """Operands of one sign, where what the split leaves out and what the tensor core cuts off only add up. Parts
+    rounded to nearest are at most 2^-8 and 2^-16 of the value, so x2 w3 + x3 w2 + x3 w3, left out, is at
+    most (2 + 2^-8) 2^-24 of a product. An accumulator takes 16 values of K at a time and is promoted every 256: its at
+    most 16 additions each cut off less than 2^-23 of it (the first adds to nothing: none at K up to 16, whose
+    products are exact). The corrections, at most 2^-6 of the sum, add a 64th of that for five times as many additions. Two
+    roundings to promote the first 256 values, one more for each further 256."""
+    x = torch.full((M, K), value, device="cuda")
+    w = torch.full((130, K), value, device="cuda")
+    x[1::2] *= -0.75  # whole rows: every sum keeps one sign
+    w[1::3] *= 1.25
+    y = linear(ctx, x, w, "f32").double()
+    want = x.double() @ w.double().T
+    steps = min(-(-K // 16), 16) - 1
+    tol = (2 + 2.0 ** -8 + 2 * (steps * 69 / 64 + 5 / 64) + 2 + K / 256) * 2.0 ** -24
+    worst = float(((y - want).abs() / want.abs()).max())
+    assert worst <= tol, f"{worst * 2 ** 24} of {tol * 2 ** 24} in units of 2^-24"
+
+
+@pytest.mark.parametrize("M", [20, 300])
+def test_f32_parts_near_the_largest_value(ctx, M):
+    """A value whose leading part would round to infinity keeps a finite one."""
+    top = torch.finfo(torch.float32).max
+    x = torch.tensor([top, -top, top * (1 - 2.0 ** -9), 3.3961775e38], device="cuda").repeat(M // 4)[:, None].contiguous()
+    w = torch.tensor([1.0, 0.5, -0.25, 2.0 ** -100, 1 - 2.0 ** -24], device="cuda")[:, None].contiguous()
+    y = linear(ctx, x, w, "f32").double()
+    want = x.double() @ w.double().T
+    assert bool(y.isfinite().all())
+    assert float(((y - want).abs() / want.abs()).max()) <= 2.0 ** -21  # cut at the top of the range: 2^-7, 2^-15 parts
