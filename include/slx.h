@@ -221,9 +221,10 @@ slx_status slx_attention(slx_ctx* ctx, const int64_t* q, const int64_t* k, const
  * may be freed afterwards; the handle itself must outlive graphs that captured its calls. dtype is the type of x,
  * residual and y: F32 takes weights of any GGUF type slx_dequantize decodes, F16 and BF16 weights of their
  * own type. d_gate NULL: no gate. Sums and the epilogue are fp32, rounded once to dtype.
- * An F32 product of more than 8 rows runs on the tensor cores from three bf16 parts of every value, each rounded to
- * nearest: a finite result is as exact as an fp32 sum (one within 2^-7 of the largest value may end infinite), an
- * infinite x or w gives an infinity or a NaN.
+ * An F32 product of up to 4 rows sums fp32 products; one of more than 16 runs on the tensor cores from three bf16
+ * parts of every value, each rounded to nearest; between them the weights' number decides. Either way a finite result
+ * is as exact as an fp32 sum (on the tensor cores one within 2^-7 of the largest value may end infinite), and
+ * infinities and NaN of x and w give what fp32 arithmetic gives.
  * slx_linear_device (device pointers): x [M][K], residual (nullable) and y [M][N] with row strides in elements, at least the
  * row's width; y may be the residual's buffer (same stride) and must not overlap x otherwise. Any M >= 0.
  * Results do not change from call to call. A bounded wait that gave up is reported by slx_ctx_status

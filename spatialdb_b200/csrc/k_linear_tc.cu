@@ -14,7 +14,9 @@
 // either sign. (Parts cut off instead of rounded leave out up to 2^-21 |x| |w|, all of the product's sign: 7.8 x 2^-24 of
 // 1.0078^2.) The tensor core truncates when it adds to an accumulator, which biases long sums, so every 256 values
 // of K both accumulators are added to fp32 registers (rounded to nearest) and started anew. x1 w1 may pass the sum it
-// stands for by 2^-7 of it: a sum within 2^-7 of the largest finite value may end infinite.
+// stands for by 2^-7 of it: a sum within 2^-7 of the largest finite value may end infinite. An infinity or NaN is all
+// in its first part, so x1 w1 alone is what fp32 makes of it, and the corrections, where it meets the zeros of exact
+// bf16 values, are left out of a sum that is not finite.
 //
 // Three forms, the cheapest by an estimate of its cycles (choose):
 //   ONE   one tile at a time. A cluster of S = 1, 2, 4 or 8 CTAs shares the tile, each with a range of the K
@@ -694,6 +696,13 @@ k_linear_tc(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUt
                             const uint32_t at = tbase + (buf * Sh::ACC + 2 * v) * NT + c;
                             tmem_cols<SLAB>(at, a);
                             tmem_cols<SLAB>(at + NT, k);
+                            float all = a[0];
+#pragma unroll
+                            for (int j = 1; j < SLAB; j++) all += a[j];
+                            if (!isfinite(all)) {  // some sum may not be finite: it keeps clear of the corrections
+#pragma unroll
+                                for (int j = 0; j < SLAB; j++) k[j] = isfinite(a[j]) ? k[j] : 0.0f;
+                            }
 #pragma unroll
                             for (int j = 0; j < SLAB; j++) acc[v][c + j] = chunks ? acc[v][c + j] + (a[j] + k[j]) : a[j] + k[j];
                         }

@@ -68,3 +68,51 @@ def test_f32_parts_near_the_largest_value(ctx, M):
     want = x.double() @ w.double().T
     assert bool(y.isfinite().all())
     assert float(((y - want).abs() / want.abs()).max()) <= 2.0 ** -21  # cut at the top of the range: 2^-7, 2^-15 parts
+
+
+# ---- infinities ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("K,exact16", [(200, True), (200, False), (700, True)])
+@pytest.mark.parametrize("M", [1, 3, 6, 12, 40, 300, 2000])
+def test_f32_infinities(ctx, M, K, exact16, gated):
+    """Infinities and NaN in x and w end where fp32 arithmetic takes them, whichever kernel a call's sizes pick: an
+    infinity of the product's sign, NaN against a zero or an infinity of the other sign. Weights that are exact in
+    bf16 have zeros for their second and third parts."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(M + K)
+    x = torch.randn(M, K, generator=gen, device="cuda")
+    w = torch.randn(150, K, generator=gen, device="cuda") / math.sqrt(K)
+    g = torch.rand(150, K, generator=gen, device="cuda") if gated else None
+    if exact16:
+        x, w = x.bfloat16().float(), w.bfloat16().float()
+    inf, nan = float("inf"), float("nan")
+    x[M // 2, K // 2] = inf
+    x[M // 3, 5] = -inf
+    w[4, K // 2] = 0.0
+    w[9, 6] = inf
+    w[11, 5] = -inf
+    w[20, 1] = nan
+    if M > 3:
+        x[M - 1, 2], x[M - 1, K - 1] = inf, inf
+        x[0, 3] = nan
+    y = linear(ctx, x, w, "f32", act=slx.ACT_RELU if gated else 0, gate=g)
+
+    def product(w):
+        p, kinds = x.double()[:, None, :] * w.double()[None], (inf, -inf)
+        up, down = ((p == k).any(-1) for k in kinds)
+        s = torch.where(p.isfinite(), p, 0.0).sum(-1)
+        s = torch.where(up, inf, torch.where(down, -inf, s))
+        return torch.where(p.isnan().any(-1) | (up & down), nan, s)
+
+    want = product(w)
+    if gated:
+        v = product(g)
+        want = torch.where(v < 0, 0.0, v) * want  # a NaN stays one
+    odd = ~want.isfinite()
+    assert int(odd.sum()) >= 150
+    assert torch.equal(y.isnan(), want.isnan())
+    inf_at = want.isinf()
+    assert torch.equal(y[inf_at].double(), want[inf_at])
+    assert bool(y[~odd].isfinite().all())
