@@ -59,3 +59,18 @@ def test_rounded_bf16_parts_sum_to_the_value():
     left = (x2 * w3 + x3 * w2 + x3 * w3) / (x.astype(np.float64) * w)
     assert np.abs(left).max() <= 2.0 ** -23.9
     assert abs(left.mean()) <= 6 * left.std() / math.sqrt(left.size)
+
+
+def test_erfc_polynomials():
+    """erfc(z) = e^(-z^2) t P(t), t = 1 / (1 + a z), with the kernels' constants: the relative errors their comment states,
+    over the z whose results the output's type can hold."""
+    text = source("slx_linear_dev.cuh")
+    a32, a16 = (float(np.float32(x)) for x in re.search(r"A = F \? ([0-9.]+)f : ([0-9.]+)f", text).groups())
+    for name, a, top, bound in (("c32", a32, 10.2, 2.7e-8), ("c16", a16, 9.6, 2.0 ** -17.5)):
+        c = [float(np.float32(x.strip(" f"))) for x in re.search(name + r"\[\d+\] = \{(.*?)\}", text).group(1).split(",")]
+        worst = 0.0
+        for z in np.linspace(0.0, top, 20001):
+            t = 1.0 / (1.0 + a * z)
+            p = t * sum(v * t ** i for i, v in enumerate(c))
+            worst = max(worst, abs(p * math.exp(-z * z) / math.erfc(z) - 1.0))
+        assert worst <= bound, (name, worst)

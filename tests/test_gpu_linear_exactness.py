@@ -116,3 +116,70 @@ def test_f32_infinities(ctx, M, K, exact16, gated):
     inf_at = want.isinf()
     assert torch.equal(y[inf_at].double(), want[inf_at])
     assert bool(y[~odd].isfinite().all())
+
+
+# ---- activations ---------------------------------------------------------------------------------------
+
+
+def act64(v, act):
+    """Each activation as v times its factor, the factor formed without cancellation."""
+    if act == "silu":
+        return v * torch.special.expit(v)
+    if act == "gelu_tanh":
+        return v * torch.special.expit(2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3))
+    return 0.5 * v * torch.special.erfc(-v / math.sqrt(2))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("M", [1, 12, 40, 700])
+def test_activation_tails(ctx, dtype, act, M):
+    """act(v) for v given exactly (K = 1, x = 1), held to a tolerance relative to the output, so that the negative
+    tails, where it is small, count as much as the rest. With u = 2^-24:
+
+    The exponential of s (s = v, or GELU-tanh's 2 sqrt(2 / pi) (v + 0.044715 v^3)): CUDA's expf is good to 2 units of its
+    last place (4 u), __expf, which 16-bit outputs may take, to 2 + 1.173 |s| units, 2 u each; s itself is off by two
+    rounded constants and four roundings, 5 u at most, which the exponential makes 5 u |s|. Sum, quotient (its fast form: two
+    units), product: 6 u.
+
+    GELU-erf's tail is v e^(-v^2 / 2) t P(t) with t = 1 / (1 + a z). The exponent is off by one rounding, v^2 / 2 u of the
+    exponential, itself 4 u or (2 + 1.173 v^2 / 2) 2 u. t is off by 3.5 u (z 1.5, sum and quotient; a hardware reciprocal
+    1 more), of which t P(t) makes at most 3.8 times as much (its logarithm's slope in log t, erfc's 2 / sqrt(pi) over
+    a = 0.3 at z = 0, falling to 1). Horner's steps: the terms' sizes add up to 2.5 P(t) at most, three roundings each: 7.5 u. P
+    itself: u / 2 in f32, 2^-17.5 = 91 u for 16-bit outputs. Products 3 u. Together (28.3 + v^2 / 2) u and
+    (91 + 32 + 1.7 v^2) u. Above zero v (1 - tail) is better than that.
+
+    Then half a step of the type, and below its normal range half its smallest step (f32: |v| times it, and whole: the
+    exponential itself lies there)."""
+    code, dt = TYPES[dtype]
+    v = torch.cat([torch.linspace(-14, 14, 2801), torch.linspace(-104, -13, 911), torch.linspace(14, 100, 44),
+                   torch.tensor([0.0, -0.0, 1e-30, -1e-30, 6e4, -6e4, 2.0 ** -14, -(2.0 ** -14)])]).to(dt).cuda()
+    if dtype != "f16":
+        v = torch.cat([v, torch.tensor([3e38, -3e38, 1e19, -1e19, 2e13, -2e13], device="cuda").to(dt)])
+    y = linear(ctx, torch.ones(M, 1, dtype=dt, device="cuda"), v[:, None].contiguous(), dtype, act=ACTS[act])
+    assert torch.equal(y, y[:1].expand_as(y))
+    a = v.double()
+    want, u = act64(a, act), 2.0 ** -24
+    s = (a if act == "silu" else 2 * math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)).abs().clamp_max(105)
+    if act == "gelu_erf":
+        sq = a.square().clamp_max(220)
+        rel = (28.3 + sq / 2 if dtype == "f32" else 91 + 32 + 1.7 * sq) * u
+    else:
+        rel = ((5 * s if act == "gelu_tanh" else 0) + (4 if dtype == "f32" else 2 * (2 + 1.173 * s)) + 6) * u
+    least = {"f32": 2.0 ** -149 * (a.abs().clamp_max(105) + 1), "f16": 2.0 ** -25, "bf16": 2.0 ** -134}[dtype]
+    tol = rel * want.abs()
+    tol = tol + torch.finfo(dt).eps / 2 * (want.abs() + tol) * (dtype != "f32") + least
+    d = (y[0].double() - want).abs()
+    at = int((d / tol).argmax())
+    assert bool((d <= tol).all()), f"act({float(a[at])}) = {float(y[0, at])}, {float(want[at])} wanted: {float(d[at] / tol[at])} of the tolerance"
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("M", [2, 40])
+def test_activations_of_what_is_not_finite(ctx, dtype, act, M):
+    """+infinity is kept, a NaN stays one, and -infinity is the formula's -infinity times zero."""
+    code, dt = TYPES[dtype]
+    w = torch.tensor([float("inf"), -float("inf"), float("nan"), 1.0], device="cuda").to(dt)[:, None].contiguous()
+    y = linear(ctx, torch.ones(M, 1, dtype=dt, device="cuda"), w, dtype, act=ACTS[act])
+    assert bool((y[:, 0] == float("inf")).all()) and bool(y[:, 1:3].isnan().all()) and bool(y[:, 3].isfinite().all())
