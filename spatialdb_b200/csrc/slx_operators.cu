@@ -14,6 +14,7 @@
 #include "slx_kernels.h"
 #include "slx_linear.h"
 #include "slx_qk_rope.h"
+#include "slx_rows.h"
 
 using namespace slx;
 
@@ -226,6 +227,9 @@ slx_status slx_linear_device(slx_linear* l, const slx_linear_args* a) {
         return set_err(ctx, SLX_EINVAL, "rows not aligned to %d bytes", e);
     if (M > (1 << 30) || (M + 31) / 32 * p.tiles_n() > (1ll << 27) || a->ldx > (1ll << 36))
         return set_err(ctx, SLX_EINVAL, "M %lld with N %d, row stride %lld", (long long)M, p.N, (long long)a->ldx);
+    if (rows_overlap(a->x, a->ldx, p.K, a->y, a->ldy, p.N, M, e)) return set_err(ctx, SLX_EINVAL, "y overlaps x");
+    if ((a->residual != a->y || a->ldr != a->ldy) && rows_overlap(a->residual, a->ldr, p.N, a->y, a->ldy, p.N, M, e))
+        return set_err(ctx, SLX_EINVAL, "y overlaps the residual without being it");
     OnDevice on(ctx->device);
     CK(on.err);
     cudaStream_t st = pick(ctx, a->stream);
@@ -376,6 +380,14 @@ slx_status slx_qk_norm_rope_device(slx_qk_norm* h, const slx_qk_args* a) {
         return set_err(ctx, SLX_ERANGE, "sequence length %lld exceeds the RoPE table (%d rows)", (long long)T, r->rows);
     if (M > (1ll << 32) / (h->heads + h->kv_heads))
         return set_err(ctx, SLX_EINVAL, "M %lld rows of %d heads", (long long)M, h->heads + h->kv_heads);
+    auto meet = [&](const void* x, int64_t ldx, int64_t wx, const void* y, int64_t ldy, int64_t wy) {
+        return wx && wy && rows_overlap(x, ldx, wx, y, ldy, wy, M, e);
+    };
+    if (((a->qo != a->q || a->ldqo != a->ldq) && meet(a->q, a->ldq, nq, a->qo, a->ldqo, nq)) ||
+        ((a->ko != a->k || a->ldko != a->ldk) && meet(a->k, a->ldk, nk, a->ko, a->ldko, nk)) ||
+        meet(a->q, a->ldq, nq, a->ko, a->ldko, nk) || meet(a->k, a->ldk, nk, a->qo, a->ldqo, nq) ||
+        meet(a->qo, a->ldqo, nq, a->ko, a->ldko, nk))
+        return set_err(ctx, SLX_EINVAL, "an output overlaps the inputs, or the other output, without being its input");
     OnDevice on(ctx->device);
     CK(on.err);
     cudaStream_t st = pick(ctx, a->stream);

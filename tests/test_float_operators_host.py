@@ -1,7 +1,9 @@
 """Host-side checks of the float operators' sources and helpers that need no device."""
+import itertools
 import math
 import os
 import re
+import subprocess
 
 import numpy as np
 
@@ -74,3 +76,31 @@ def test_erfc_polynomials():
             p = t * sum(v * t ** i for i, v in enumerate(c))
             worst = max(worst, abs(p * math.exp(-z * z) / math.erfc(z) - 1.0))
         assert worst <= bound, (name, worst)
+
+
+def test_overlap_of_strided_rows(tmp_path):
+    """rows_overlap against the bytes themselves, over every small arrangement of two arrays of rows."""
+    main = tmp_path / "rows.cpp"
+    main.write_text('''
+#include <cstdio>
+#include "slx_rows.h"
+int main() {
+    long long p[8];
+    while (std::scanf("%lld %lld %lld %lld %lld %lld %lld %lld", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7) == 8)
+        std::printf("%d", (int)slx::rows_overlap((void*)p[0], p[1], p[2], (void*)p[3], p[4], p[5], p[6], (int)p[7]));
+}
+''')
+    exe = str(tmp_path / "rows")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", build.CSRC, str(main), "-o", exe], check=True)
+    calls, want = [], []
+    for lda, ldb, M, e in itertools.product((3, 5), (3, 4, 5, 9), (1, 2, 3), (1, 2)):
+        for wa, wb, d in itertools.product((1, 2, 3), (1, 3), range(-20, 21)):
+            a, b = 4096, 4096 + d * e
+            at = [{p + m * ld * e + i for m in range(M) for i in range(w * e)} for p, ld, w in ((a, lda, wa), (b, ldb, wb))]
+            calls.append((a, lda, wa, b, ldb, wb, M, e))
+            want.append(bool(at[0] & at[1]))
+    big = 1 << 40  # strides past 32 bits, and nothing to read
+    calls += [(64, big, 8, 64 + big * 4, big, 8, 100, 4), (64, big, 8, 80, big, 8, 1 << 20, 4), (64, big, 8, 96, big, 8, 1 << 20, 4), (0, 8, 8, 0, 8, 8, 4, 4)]
+    want += [True, True, False, False]
+    out = subprocess.run([exe], input="\n".join(" ".join(map(str, c)) for c in calls), capture_output=True, text=True, check=True).stdout
+    assert [c == "1" for c in out] == want
