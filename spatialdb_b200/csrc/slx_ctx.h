@@ -83,9 +83,23 @@ inline int set_err(slx_ctx* c, int code, const char* fmt, ...) {
         }                                                                                        \
     } while (0)
 
+// Makes a device current for one scope and puts the caller's back.
+struct OnDevice {
+    int prev = -1;
+    cudaError_t err;
+    explicit OnDevice(int dev) {
+        err = cudaGetDevice(&prev);
+        if (err == cudaSuccess && prev != dev) err = cudaSetDevice(dev);
+        else prev = -1;
+    }
+    ~OnDevice() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
 inline cudaStream_t pick(slx_ctx* ctx, void* s) { return s ? (cudaStream_t)s : ctx->stream; }
 
-// Drops one reference; the last one frees the context.
+// Drops one reference; the last one frees the context. The current device stays what it is.
 void ctx_release(slx_ctx* ctx);
 
 }  // namespace slx

@@ -899,7 +899,7 @@ void to_float_l2(const int64_t* v, int d, int sb, float* out) {
 // order the host frees them in (a garbage-collected host may finalize the context first).
 void slx::ctx_release(slx_ctx* ctx) {
     if (ctx->refs.fetch_sub(1) != 1) return;
-    cudaSetDevice(ctx->device);
+    const OnDevice on(ctx->device);
     if (ctx->stream) cudaStreamSynchronize(ctx->stream);
     cudaFree(ctx->d_flag);
     for (auto& r : ctx->records) { cudaEventDestroy(r.a); cudaEventDestroy(r.b); }

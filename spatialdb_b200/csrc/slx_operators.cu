@@ -22,20 +22,6 @@ static_assert(SLX_DTYPE_F32 == GG_F32 && SLX_DTYPE_F16 == GG_F16 && SLX_DTYPE_BF
 
 namespace {
 
-// Makes the context's device current for one call and puts the caller's back.
-struct OnDevice {
-    int prev = -1;
-    cudaError_t err;
-    explicit OnDevice(int dev) {
-        err = cudaGetDevice(&prev);
-        if (err == cudaSuccess && prev != dev) err = cudaSetDevice(dev);
-        else prev = -1;
-    }
-    ~OnDevice() {
-        if (prev >= 0) cudaSetDevice(prev);
-    }
-};
-
 bool is_float(int dtype) { return dtype == SLX_DTYPE_F32 || dtype == SLX_DTYPE_F16 || dtype == SLX_DTYPE_BF16; }
 int width_of(int dtype) { return dtype == SLX_DTYPE_F32 ? 4 : dtype == SLX_DTYPE_Q30 ? 8 : 2; }
 

@@ -104,3 +104,44 @@ int main() {
     want += [True, True, False, False]
     out = subprocess.run([exe], input="\n".join(" ".join(map(str, c)) for c in calls), capture_output=True, text=True, check=True).stdout
     assert [c == "1" for c in out] == want
+
+
+def test_freeing_the_last_object_leaves_the_current_device(tmp_path):
+    """ctx_release, as it stands, against stand-ins of the CUDA runtime: whichever device was current still is."""
+    text = source("slx_model.cu")
+    body = text[text.index("void slx::ctx_release"):]
+    body = body[:body.index("\n}\n") + 3]
+    header = source("slx_ctx.h")
+    guard = header[header.index("struct OnDevice {"):]
+    guard = guard[:guard.index("};") + 2]
+    main = tmp_path / "release.cpp"
+    main.write_text("""
+#include <atomic>
+#include <cstdio>
+#include <vector>
+typedef int cudaError_t; enum { cudaSuccess = 0 };
+int current = 0, freed_on = -1;
+int cudaGetDevice(int* d) { *d = current; return 0; }
+int cudaSetDevice(int d) { current = d; return 0; }
+template <class T> int cudaFree(T) { freed_on = current; return 0; }
+template <class T> int cudaEventDestroy(T) { return 0; }
+template <class T> int cudaStreamSynchronize(T) { return 0; }
+template <class T> int cudaStreamDestroy(T) { return 0; }
+template <class T> int cudaMemPoolDestroy(T) { return 0; }
+template <class T> void gemm_workspace_free(T) {}
+typedef int cudaEvent_t;
+struct Record { int a, b; };
+struct slx_ctx { std::atomic<int> refs{1}; int device = 3, stream = 1, d_flag = 1, kws = 0, pool = 1;
+                 std::vector<Record> records; std::vector<int> event_pool; };
+namespace slx { void ctx_release(slx_ctx*); %s }
+using namespace slx;
+%s
+int main() {
+    current = 1;
+    slx::ctx_release(new slx_ctx());
+    std::printf("%%d %%d", current, freed_on);
+}
+""" % (guard, body))
+    exe = str(tmp_path / "release")
+    subprocess.run(["g++", "-std=c++17", str(main), "-o", exe], check=True)
+    assert subprocess.run([exe], capture_output=True, text=True, check=True).stdout == "1 3"
