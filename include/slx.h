@@ -66,9 +66,13 @@ slx_status slx_ctx_status(slx_ctx* ctx, void* stream);
  * the kernel then lets its copies and MMAs in flight finish, frees its tensor memory, returns and
  * reports SLX_ETIMEOUT, leaving the context usable. SLX_OPT_TEST_STALL_MMA (testing only): nonzero
  * makes that GEMM's MMA warp issue nothing, so its pipeline waits run out and the timeout path runs
- * without any fault; results of such calls are undefined. */
+ * without any fault; results of such calls are undefined. SLX_OPT_TEST_LINEAR_FORM (testing only): nonzero makes
+ * slx_linear_device take one form of its tensor-core kernel whatever the sizes: the width of its tiles (32, 64,
+ * 128, 256) + 1024 x mode (0 one tile a cluster, 1 pairs, 2 wide gated pairs) + 4096 x log2 of the cluster's
+ * size (mode 0: 0..3); a call that the form cannot compute is refused with SLX_EUNSUPPORTED. */
 #define SLX_OPT_WAIT_LIMIT_CYCLES 1
 #define SLX_OPT_TEST_STALL_MMA 2
+#define SLX_OPT_TEST_LINEAR_FORM 3
 slx_status slx_ctx_set_option(slx_ctx* ctx, int option, int64_t value);
 
 /* ---- GGUF ---------------------------------------------------------------------------------- */

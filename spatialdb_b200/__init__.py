@@ -28,7 +28,7 @@ from ._lib import I32P, I64P, F32P, U8P, U64P, VP
 
 (SLX_OK, SLX_EINVAL, SLX_EFORMAT, SLX_ENOTFOUND, SLX_EUNSUPPORTED, SLX_EEOF, SLX_ERANGE, SLX_EOOM, SLX_ECUDA, SLX_ETIMEOUT,
  SLX_ESCRATCH) = range(11)
-OPT_WAIT_LIMIT_CYCLES, OPT_TEST_STALL_MMA = 1, 2
+OPT_WAIT_LIMIT_CYCLES, OPT_TEST_STALL_MMA, OPT_TEST_LINEAR_FORM = 1, 2, 3
 MODEL_ENCODER, MODEL_CAUSAL, MODEL_GEMMA_ENCODER, MODEL_FLOAT_ENCODER = 0, 1, 2, 3
 DTYPE_F32, DTYPE_F16, DTYPE_Q30, DTYPE_BF16 = 0, 1, 27, 30
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU_TANH, ACT_GELU_ERF = range(5)

@@ -1073,6 +1073,14 @@ Choice choose(const Plan& p, const Call& c) {
     return best;
 }
 
+bool has_form(const Plan& p, const Choice& ch) {
+    const int planes = p.planes(), widest = (planes == 3 ? 128 : 256) / (p.gated ? 2 : 1), pair_widest = planes == 3 ? 128 : 256;
+    const bool width = ch.nt == 32 || ch.nt == 64 || ch.nt == 128 || ch.nt == 256;
+    if (ch.mode == ONE) return width && ch.nt <= std::min(widest, 128) && (!ch.log2_split || p.nkb() >= 2 << ch.log2_split);
+    if (ch.log2_split) return false;
+    return ch.mode == PAIR ? width && ch.nt <= pair_widest && ch.nt * 4 >= pair_widest : ch.mode == WIDE && p.gated && planes == 1 && ch.nt == 128;
+}
+
 size_t tc_workspace(const Plan& p, const Call& c, const Choice& ch) {
     if (tma_rows(p, c) || ch.mode == ONE) return 0;
     return (size_t)p.planes() * c.M * kp_of(p) * 2;

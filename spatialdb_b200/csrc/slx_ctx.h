@@ -33,6 +33,7 @@ struct slx_ctx {
     std::vector<ProfRecord> records;
     slx::GemmWorkspace kws;          // scratch of the kernel-level matmul entry points
     slx::WaitOptions wait;           // bounded-wait settings of the tensor-core GEMMs (slx_ctx_set_option)
+    int linear_form = 0;             // SLX_OPT_TEST_LINEAR_FORM
     std::atomic<int> refs{1};        // slx_destroy's reference plus one per live object created on it
     cudaMemPool_t pool = nullptr;    // stream-ordered scratch of the float operators, made at first use
     std::vector<cudaEvent_t> event_pool;

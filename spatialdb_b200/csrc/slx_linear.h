@@ -66,6 +66,7 @@ struct Choice {
     double cycles = 0;
 };
 Choice choose(const Plan& p, const Call& c);
+bool has_form(const Plan& p, const Choice& ch);  // whether the kernel is built for it and the sums can be split so
 size_t tc_workspace(const Plan& p, const Call& c, const Choice& ch);
 int tc(const Plan& p, const Call& c, const Choice& ch, void* ws, cudaStream_t st);
 

@@ -956,6 +956,10 @@ slx_status slx_ctx_set_option(slx_ctx* ctx, int option, int64_t value) {
         case SLX_OPT_TEST_STALL_MMA:
             ctx->wait.stall_mma = value ? 1 : 0;
             return SLX_OK;
+        case SLX_OPT_TEST_LINEAR_FORM:
+            if (value < 0 || value >= 4 * 4096) return set_err(ctx, SLX_EINVAL, "linear form %lld", (long long)value);
+            ctx->linear_form = (int)value;
+            return SLX_OK;
         default:
             return set_err(ctx, SLX_EINVAL, "unknown option %d", option);
     }

@@ -226,12 +226,19 @@ slx_status slx_linear_device(slx_linear* l, const slx_linear_args* a) {
     c.stall_mma = ctx->wait.stall_mma;
     const double macs = (double)M * p.N * p.K * (p.gated ? 2 : 1);
     const double bytes = (double)e * (M * p.K + (double)p.N * p.K * (p.gated ? 2 : 1) + M * p.N * (a->residual ? 2 : 1));
-    if (lin::few_supported(p, M)) {
+    if (!ctx->linear_form && lin::few_supported(p, M)) {
         run_k(ctx, KC_GEMV, macs, bytes, st, [&] { return lin::few(p, c, st); });
         CK(cudaGetLastError());
         return SLX_OK;
     }
-    const lin::Choice ch = lin::choose(p, c);
+    lin::Choice ch;
+    if (const int form = ctx->linear_form) {
+        ch.nt = form % 1024; ch.mode = form / 1024 % 4; ch.log2_split = form / 4096;
+        if (!lin::has_form(p, ch))
+            return set_err(ctx, SLX_EUNSUPPORTED, "linear form %d (width %d, mode %d, split %d)", form, ch.nt, ch.mode, 1 << ch.log2_split);
+    } else {
+        ch = lin::choose(p, c);
+    }
     void* ws = nullptr;
     if (const size_t need = lin::tc_workspace(p, c, ch)) {
         CK(cudaMallocFromPoolAsync(&ws, need, ctx->pool, st));
