@@ -224,7 +224,8 @@ slx_status slx_attention(slx_ctx* ctx, const int64_t* q, const int64_t* k, const
  * d_gate, d_bias and d_gate_bias (device memory, complete before the call; the biases f32[N], nullable)
  * may be freed afterwards; the handle itself must outlive graphs that captured its calls. dtype is the type of x,
  * residual and y: F32 takes weights of any GGUF type slx_dequantize decodes, F16 and BF16 weights of their
- * own type. d_gate NULL: no gate. Sums and the epilogue are fp32, rounded once to dtype.
+ * own type. d_gate NULL: no gate. Sums and the epilogue are fp32, rounded once to dtype. The tensor cores cut off what
+ * they add to a 16-bit product's sum: operands of one sign come out low by about K x 6e-9.
  * An F32 product of up to 4 rows sums fp32 products; one of more than 16 runs on the tensor cores from three bf16
  * parts of every value, each rounded to nearest; between them the weights' number decides. Either way a finite result
  * is as exact as an fp32 sum (on the tensor cores one within 2^-7 of the largest value may end infinite), and

@@ -3,15 +3,17 @@
 //
 // 16-bit, up to 16 rows: one block per 16 weight rows, its eight warps taking 64-wide K blocks in turn, two
 // at a time (everything they need is asked for before any of it is used; four at a time take the registers
-// of half the blocks: 18.3 against 16.5 us below). In the tiled layout 16 rows of a K block are 2 KB in a
+// of half the blocks: 18.3 against 16.5 us, short runs of the first figure below). In the tiled layout 16 rows of a K block are 2 KB in a
 // row; a lane loads 16-byte chunks t and t + 4 of rows g and g + 8 (g = lane / 4, t = lane % 4). A chunk's
 // eight values feed two m16n8k16 products whose K order is permuted alike on both sides (a sum does not
 // care), so weights go from memory to the matrix instruction without shared memory or shuffles; x comes from
 // cache in the same order. The tensor pipe is idle most of the time: what counts is the bytes in flight.
-// bf16 1 x 4096 x 11008: 16.5 us, 5455 GB/s; f16 8 x 4096 x 4096: 8.5 us; bf16 1 x 2048 x 16384 gated: 21.8 us,
-// 6148 GB/s.
+// The matrix instructions cut off what they add to a sum; a warp adds an eighth of K, and the eight sums are joined by
+// fp32 additions (K 8192, f16, operands of one sign: low by 6e-6; the output's half step is 2.4e-4).
+// In a loop of calls bf16 1 x 4096 x 11008 takes 17.7 us, 5100 GB/s; f16 8 x 4096 x 4096 8.5 us, 3960; bf16 1 x 2048 x
+// 16384 gated 22.1 us, 6070.
 // f32, up to 16 rows: one block per 8 weight rows (4 + 4 when gated), four consecutive K values a lane,
-// fp32 FMAs. 1 x 4096 x 11008: 29.7 us, 6076 GB/s.
+// fp32 FMAs. 1 x 4096 x 11008: 29.4 us, 6130 GB/s.
 // Both join the warps' partial sums in shared memory in a fixed order and apply the epilogue there.
 #include <algorithm>
 #include <cstdint>
@@ -267,8 +269,8 @@ void launch32(FewParams p, cudaStream_t st) {
 }  // namespace
 
 // f32 past 4 rows: the sums leave few registers for loads, and the tensor-core form, which reads six bytes a
-// weight instead of four, catches up (us here and there: 8 x 768 x 2304 4.2, 9.1; 8 x 4096 x 4096 30.8, 25.9;
-// 16 x 768 x 2304 7.8, 9.1; 10 x 8096 x 32 9.6, 24.8; 11 x 1632 x 10016 38.2, 36.2; 16 x 4096 x 4096 46.7, 25.9).
+// weight instead of four, catches up (us here and there: 8 x 768 x 2304 4.2, 9.1; 8 x 4096 x 4096 30.8, 24.2;
+// 16 x 768 x 2304 7.8, 9.1; 10 x 8096 x 32 9.6, 24.8; 11 x 1632 x 10016 38.2, 36.2; 16 x 4096 x 4096 46.7, 24.2).
 bool few_supported(const Plan& p, int64_t M) {
     if (p.dtype != DT_F32 || M <= 4) return M <= 16;
     const int64_t weights = (int64_t)p.N * p.K * (p.gated ? 2 : 1);

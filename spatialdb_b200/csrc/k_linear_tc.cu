@@ -12,11 +12,19 @@
 // |x2| <= 2^-8 |x| and |x3| <= 2^-17 |x|. x1 w1 goes to one accumulator, the corrections x1 w2 + x2 w1 + x2 w2 +
 // x1 w3 + x3 w1 (at most 2^-6.9 of it) to another; x2 w3 + x3 w2 + x3 w3, left out, is at most 2^-23.9 |x| |w| and of
 // either sign. (Parts cut off instead of rounded leave out up to 2^-21 |x| |w|, all of the product's sign: 7.8 x 2^-24 of
-// 1.0078^2.) The tensor core truncates when it adds to an accumulator, which biases long sums, so every 256 values
+// 1.0078^2.) The tensor core truncates what it adds, which biases long sums, so every 256 values
 // of K both accumulators are added to fp32 registers (rounded to nearest) and started anew. x1 w1 may pass the sum it
 // stands for by 2^-7 of it: a sum within 2^-7 of the largest finite value may end infinite. An infinity or NaN is all
 // in its first part, so x1 w1 alone is what fp32 makes of it, and the corrections, where it meets the zeros of exact
 // bf16 values, are left out of a sum that is not finite.
+//
+// 16 bits: the sums stay in the truncating accumulator over all of K. An addition aligns 16 products and the sum to the
+// largest of them, keeps 25 bits of each and 24 of the result (measured): operands of one sign come out low by about
+// K x 6e-9, 1.2e-5 at K = 2048 and 5e-5 at 8192 (a sixth of that with random signs), where half a step of an f16 output
+// is 2.4e-4 to 4.9e-4 and of a bf16 output eight times that. Against 64 bits the outputs' error stays that of their
+// rounding (bf16 512 x 2048 x 16384 gated: 1.66e-3, as with sums in fp32 FMAs, against which 0.2 % of the outputs round
+// the other way). Promoting the sums as in f32 would take 64 registers a thread with 256 columns a tile; of 96 the
+// epilogue uses all.
 //
 // Three forms, the cheapest by an estimate of its cycles (choose):
 //   ONE   one tile at a time. A cluster of S = 1, 2, 4 or 8 CTAs shares the tile, each with a range of the K
@@ -36,11 +44,12 @@
 // epilogue's staging (K 768): 543 cycles a block measured without a concurrent epilogue, 713 with one. Gated, 810
 // (K 2048); with 128 columns of each array in accumulators of their own, the form before, 950.
 // Leaving out the loads of either operand changes the times by 2 to 8 %.
-// Measured (device time, L2 cold inputs; 1654.5 TFLOP/s is the card's measured cuBLAS rate): bf16 8192^3 703 us,
-// 1565 TFLOP/s; 4096 x 4096 x 11008 with bias, GELU and residual 276 us, 1340; 512 x 2048 x 16384 gated 59 us,
-// 1165; 8192 x 768 x 2304 27.3 us, 1064; f32 8192 x 768 x 2304 147 us, 197 (1180 of bf16 products), 512 x
-// 2048 x 8192 gated 169 us, 203 (one array's rows a tile, the form before: 278); f16 129 x 1001 x 1111 8.0 us. Under
-// the power cap of a long loop 4096 x 4096 x 11008 takes 312, the gated product 70 and the f32 one 164 us.
+// Measured in loops of calls, inputs larger than L2, the large products at the power cap (sustained cuBLAS bf16 is 1391.3
+// TFLOP/s): bf16 8192^3 838 us, 1312 TFLOP/s; 4096 x 4096 x 11008 with bias, GELU and residual 312 us, 1184; 512 x 2048 x
+// 16384 gated 71 us, 970; 8192 x 768 x 2304 32.7 us, 887; f32 8192 x 768 x 2304 165 us, 176 (1057 of bf16 products), 512
+// x 2048 x 8192 gated 200 us, 172 (one array's rows a tile, the form before, took 1.6 times as long); f16 129 x 1001 x
+// 1111 7.9 us. In short runs, above the sustained clock: 703, 276, 59, 27.3, 147 and 169 us. Tensor pipe active (ncu): 79 %
+// at bf16 2048 x 4096 x 8192, 66 % gated, 52 % at 8192 x 768 x 2304, 67 % in f32.
 // Every mbarrier wait is bounded.
 #include <cuda.h>
 

@@ -3,7 +3,8 @@
 // Float: for a head row x of hd values, s = 1 / sqrt(sum x^2 / hd + eps), u_j = x_j s w_j; the pair
 // (u_p, u_{p+h}), p < h, becomes (u_p c - u_{p+h} s', u_p s' + u_{p+h} c) with (c, s') the table's entry of the
 // row's position; values past 2 h keep u. All in fp32 from the loaded values to the one rounding at
-// the store. Q30: RmsNormRow, then ApplyRoPE, on int64 values.
+// the store; the root and its reciprocal are one rsqrtf, good to two units of 2^-23 for each head. Q30: RmsNormRow, then
+// ApplyRoPE, on int64 values.
 //
 // Both are bound by memory at many rows (every value is read and written once, the table's row once
 // per token) and by latency at one token. A pair's two values belong to one lane, so the rotation

@@ -42,10 +42,12 @@ def linear(ctx, x, w, dtype, act=0, gate=None):
 def test_f32_products_of_one_sign(ctx, M, K, value):
     """Operands of one sign, where what the split leaves out and what the tensor core cuts off only add up. Parts
     rounded to nearest are at most 2^-8 and 2^-16 of the value, so x2 w3 + x3 w2 + x3 w3, left out, is at
-    most (2 + 2^-8) 2^-24 of a product. An accumulator takes 16 values of K at a time and is promoted every 256: its at
-    most 16 additions each cut off less than 2^-23 of it (the first adds to nothing: none at K up to 16, whose
-    products are exact). The corrections, at most 2^-6 of the sum, add a 64th of that for five times as many additions. Two
-    roundings to promote the first 256 values, one more for each further 256."""
+    most (2 + 2^-8) 2^-24 of a product. An addition takes 16 products into an accumulator, which is promoted every 256
+    values of K; it aligns them to the largest term, keeps 25 bits of each and 24 of the sum. Products of 8-bit parts of
+    like size keep all their 16 bits beside a sum of up to 256 of them, so each addition of x1 w1 after the first (which
+    adds to nothing) cuts off less than 2^-23 of the sum. The corrections, at most 2^-6.9 of it, lose up to 16 x 2^-25 + 2^-23
+    of themselves in each of five times as many additions: 0.21 x 2^-23 of the sum for 16 values. Two roundings to promote
+    the first 256 values, one more for each further 256."""
     x = torch.full((M, K), value, device="cuda")
     w = torch.full((130, K), value, device="cuda")
     x[1::2] *= -0.75  # whole rows: every sum keeps one sign
@@ -53,7 +55,7 @@ def test_f32_products_of_one_sign(ctx, M, K, value):
     y = linear(ctx, x, w, "f32").double()
     want = x.double() @ w.double().T
     steps = min(-(-K // 16), 16) - 1
-    tol = (2 + 2.0 ** -8 + 2 * (steps * 69 / 64 + 5 / 64) + 2 + K / 256) * 2.0 ** -24
+    tol = (2 + 2.0 ** -8 + 2 * (steps + 0.21 * (steps + 1)) + 2 + K / 256) * 2.0 ** -24
     worst = float(((y - want).abs() / want.abs()).max())
     assert worst <= tol, f"{worst * 2 ** 24} of {tol * 2 ** 24} in units of 2^-24"
 
