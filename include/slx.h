@@ -230,9 +230,9 @@ slx_status slx_attention(slx_ctx* ctx, const int64_t* q, const int64_t* k, const
  * parts of every value, each rounded to nearest; between them the weights' number decides. Either way a finite result
  * is as exact as an fp32 sum (on the tensor cores one within 2^-7 of the largest value may end infinite), and
  * infinities and NaN of x and w give what fp32 arithmetic gives.
- * slx_linear_device (device pointers): x [M][K], residual (nullable) and y [M][N] with row strides in elements, at least the
- * row's width. y may be the residual (same pointer and stride); one that overlaps x, or the residual otherwise, is
- * refused. Any M >= 0.
+ * slx_linear_device (device pointers): x [M][K], residual (nullable) and y [M][N] with row strides in elements, at
+ * least the row's width. y may be the residual (same pointer and, for several rows, stride); one that overlaps x, or
+ * the residual otherwise, is refused. Any M >= 0.
  * Results do not change from call to call. A bounded wait that gave up is reported by slx_ctx_status
  * (SLX_ETIMEOUT). info: dtype, N, K, act, gated, device bytes held. */
 typedef struct slx_linear slx_linear;
@@ -262,10 +262,10 @@ slx_status slx_linear_device(slx_linear* l, const slx_linear_args* args);
  * slx_qk_norm_prepare: one layer's heads and norm weights (d_wq, d_wk [head_dim] in device memory, f32, or
  * int64 for Q30; NULL: that side is rotated only; complete before the call, copied). rot_dim <= head_dim (Q30: equal, eps 0).
  * slx_qk_norm_rope_device: q [M][heads * head_dim] to qo, k [M][kv_heads * head_dim] to ko, row strides in
- * elements, at least the row's width; an output may be its input (same pointer and stride), and is refused where it
- * overlaps an input or the other output otherwise. Row m stands at pos[m], or at m % T when pos is NULL. A
- * position of -1 leaves the row's outputs as they were; another one outside the table does too and is reported
- * by slx_ctx_status (SLX_ERANGE). heads or kv_heads may be 0 (its pointers are not read). A table may be freed
+ * elements, at least the row's width; an output may be its input (same pointer and, for several rows, stride), and
+ * is refused where it overlaps an input or the other output otherwise. Row m stands at pos[m], or at m % T when
+ * pos is NULL. A position of -1 leaves the row's outputs as they were; another one outside the table does too and
+ * is reported by slx_ctx_status (SLX_ERANGE). heads or kv_heads may be 0 (its pointers are not read). A table may be freed
  * before the layers that use it. */
 typedef struct slx_rope slx_rope;
 typedef struct slx_qk_norm slx_qk_norm;

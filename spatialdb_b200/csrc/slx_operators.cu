@@ -214,7 +214,7 @@ slx_status slx_linear_device(slx_linear* l, const slx_linear_args* a) {
     if (M > (1 << 30) || (M + 31) / 32 * p.tiles_n() > (1ll << 27) || a->ldx > (1ll << 36))
         return set_err(ctx, SLX_EINVAL, "M %lld with N %d, row stride %lld", (long long)M, p.N, (long long)a->ldx);
     if (rows_overlap(a->x, a->ldx, p.K, a->y, a->ldy, p.N, M, e)) return set_err(ctx, SLX_EINVAL, "y overlaps x");
-    if ((a->residual != a->y || a->ldr != a->ldy) && rows_overlap(a->residual, a->ldr, p.N, a->y, a->ldy, p.N, M, e))
+    if ((a->residual != a->y || (M > 1 && a->ldr != a->ldy)) && rows_overlap(a->residual, a->ldr, p.N, a->y, a->ldy, p.N, M, e))
         return set_err(ctx, SLX_EINVAL, "y overlaps the residual without being it");
     OnDevice on(ctx->device);
     CK(on.err);
@@ -376,8 +376,8 @@ slx_status slx_qk_norm_rope_device(slx_qk_norm* h, const slx_qk_args* a) {
     auto meet = [&](const void* x, int64_t ldx, int64_t wx, const void* y, int64_t ldy, int64_t wy) {
         return wx && wy && rows_overlap(x, ldx, wx, y, ldy, wy, M, e);
     };
-    if (((a->qo != a->q || a->ldqo != a->ldq) && meet(a->q, a->ldq, nq, a->qo, a->ldqo, nq)) ||
-        ((a->ko != a->k || a->ldko != a->ldk) && meet(a->k, a->ldk, nk, a->ko, a->ldko, nk)) ||
+    if (((a->qo != a->q || (M > 1 && a->ldqo != a->ldq)) && meet(a->q, a->ldq, nq, a->qo, a->ldqo, nq)) ||
+        ((a->ko != a->k || (M > 1 && a->ldko != a->ldk)) && meet(a->k, a->ldk, nk, a->ko, a->ldko, nk)) ||
         meet(a->q, a->ldq, nq, a->ko, a->ldko, nk) || meet(a->k, a->ldk, nk, a->qo, a->ldqo, nq) ||
         meet(a->qo, a->ldqo, nq, a->ko, a->ldko, nk))
         return set_err(ctx, SLX_EINVAL, "an output overlaps the inputs, or the other output, without being its input");

@@ -70,3 +70,21 @@ def test_qk_norm_rope(ctx):
     torch.cuda.synchronize()
     m = (H + KV) * hd
     assert torch.equal(x[:, :m], o[:, :m]) and torch.equal(x[:, m:], kept[:, m:])
+
+
+def test_one_row_has_no_stride(ctx):
+    """A single row in place, whatever the strides say."""
+    w = (torch.randn(64, 64, device="cuda") / 8).to(F16)
+    x, r = torch.randn(1, 64, device="cuda").to(F16), torch.randn(1, 64, device="cuda").to(F16)
+    y = torch.empty_like(x)
+    q, k = torch.randn(1, 256, device="cuda").to(F16), torch.randn(1, 128, device="cuda").to(F16)
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    torch.cuda.synchronize()
+    op = slx.Linear(slx.DTYPE_F16, w.data_ptr(), w.numel() * 2, slx.DTYPE_F16, 64, 64, ctx=ctx)
+    op.apply_device(x.data_ptr(), 1, y.data_ptr(), d_residual=r.data_ptr(), stream=slx.STREAM_LEGACY)
+    op.apply_device(x.data_ptr(), 1, r.data_ptr(), ldo=100, d_residual=r.data_ptr(), stream=slx.STREAM_LEGACY)
+    qk = slx.QkNormRope(slx.RopeTable(8, 64, ctx=ctx), slx.DTYPE_F16, 4, 2, 64)
+    for a, b, s in ((qo, ko, {}), (q, k, dict(ldq=512, ldk=512))):
+        qk.apply_device(q.data_ptr(), k.data_ptr(), 1, a.data_ptr(), b.data_ptr(), stream=slx.STREAM_LEGACY, **s)
+    torch.cuda.synchronize()
+    assert torch.equal(r, y) and torch.equal(q, qo) and torch.equal(k, ko)
